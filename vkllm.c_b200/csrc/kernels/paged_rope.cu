@@ -1,0 +1,185 @@
+// RoPE of new tokens with their key and value rows written into a paged cache.
+//
+//   (a, b) -> (a cos t - b sin t, a sin t + b cos t),  t = position * base^(-2w / hd),  pairs (2w, 2w + 1)
+//
+// on q (to q_out) and k (to the slot's key row); v is copied to the slot's value row. The pairs are
+// those of VKLLM_OP_ROPE. Every element is read and written once, so a long call is bound by HBM and a
+// short one by latency.
+//
+// Angles: fp32 loses the angle of far positions (at position 200000 the rounding of position * frequency
+// alone is 8e-3 radians). The frequency is kept as a fraction of a turn in 64-bit fixed point,
+// f = base^(-2w / hd) / (2 pi) < 2^-2, so position * f modulo 2^64 is the exact fraction of the last turn for the
+// rounded f: an error of at most position * 2^-64 turns, and no range reduction. sincospif takes it
+// from there in fp32.
+//
+// Each thread owns one 16-byte piece of a head (4 or 2 pairs), so its sines and cosines serve every head
+// that it walks over.
+#include <cmath>
+
+#include "paged.cuh"
+#include "../runtime/internal.h"
+
+namespace vkb
+{
+namespace
+{
+
+constexpr uint32_t kRopeThreads = 256;
+
+struct RopeArgs
+{
+    vkllm_b200_paged_kv kv;
+    const void *q, *k, *v;
+    void *q_out;
+    uint64_t q_stride, k_stride, v_stride, q_out_stride; // elements
+    const uint32_t *positions, *slots;
+    uint32_t n_tokens, heads;
+    uint32_t *status;
+    uint64_t turns[128]; // base^(-2w / hd) / (2 pi) * 2^64
+};
+
+template <typename T> struct Piece; // 16 bytes as fp32 pairs
+template <> struct Piece<__half>
+{
+    static constexpr int kPairs = 4;
+    __device__ static void load(const uint4 &r, float2 (&p)[4])
+    {
+        const __half2 *h = reinterpret_cast<const __half2 *>(&r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            p[i] = __half22float2(h[i]);
+    }
+    __device__ static uint4 store(const float2 (&p)[4])
+    {
+        uint4 r;
+        __half2 *h = reinterpret_cast<__half2 *>(&r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            h[i] = __floats2half2_rn(p[i].x, p[i].y);
+        return r;
+    }
+};
+template <> struct Piece<float>
+{
+    static constexpr int kPairs = 2;
+    __device__ static void load(const uint4 &r, float2 (&p)[2])
+    {
+        p[0] = make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
+        p[1] = make_float2(__uint_as_float(r.z), __uint_as_float(r.w));
+    }
+    __device__ static uint4 store(const float2 (&p)[2])
+    {
+        return make_uint4(__float_as_uint(p[0].x), __float_as_uint(p[0].y), __float_as_uint(p[1].x),
+                          __float_as_uint(p[1].y));
+    }
+};
+
+// Block: a multiple of the pieces of a head; grid.x: tokens, grid.y: shares of the token's rows (q heads, then key heads,
+// then value heads).
+template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_rope_write(const RopeArgs a)
+{
+    constexpr int P = Piece<T>::kPairs, E = 2 * P;
+    const uint32_t t = blockIdx.x, slot = a.slots[t];
+    if (slot == VKLLM_B200_NO_SLOT)
+        return;
+    const uint32_t page = slot / a.kv.page_rows, row = slot % a.kv.page_rows;
+    if (page >= a.kv.n_pages)
+    {
+        if (threadIdx.x == 0 && blockIdx.y == 0)
+            atomicOr(a.status, (uint32_t)VKLLM_B200_PAGED_BAD_SLOT);
+        return;
+    }
+    const uint32_t hd = a.kv.head_dim, pieces = hd / E, piece = threadIdx.x % pieces, lanes = blockDim.x / pieces;
+    const uint64_t pos = a.positions[t];
+    float cs[P], sn[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+    {
+        // half turns in [-1, 1)
+        const float half_turns = __ll2float_rn((long long)(pos * a.turns[piece * P + i])) * 0x1p-63f;
+        sincospif(half_turns, &sn[i], &cs[i]);
+    }
+    const uint32_t H = a.heads, K = a.kv.kv_heads, rows = H + 2 * K, off = piece * E;
+    const uint64_t cache = page * a.kv.page_stride + row * a.kv.row_stride + off;
+    for (uint32_t r = blockIdx.y * lanes + threadIdx.x / pieces; r < rows; r += gridDim.y * lanes)
+    {
+        const T *src;
+        T *dst;
+        if (r < H)
+        {
+            src = (const T *)a.q + t * a.q_stride + (uint64_t)r * hd + off;
+            dst = (T *)a.q_out + t * a.q_out_stride + (uint64_t)r * hd + off;
+        }
+        else if (r < H + K)
+        {
+            src = (const T *)a.k + t * a.k_stride + (uint64_t)(r - H) * hd + off;
+            dst = (T *)a.kv.k + cache + (r - H) * a.kv.head_stride;
+        }
+        else
+        {
+            src = (const T *)a.v + t * a.v_stride + (uint64_t)(r - H - K) * hd + off;
+            dst = (T *)a.kv.v + cache + (r - H - K) * a.kv.head_stride;
+        }
+        uint4 x = *reinterpret_cast<const uint4 *>(src);
+        if (r < H + K)
+        {
+            float2 p[P];
+            Piece<T>::load(x, p);
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                p[i] = make_float2(cs[i] * p[i].x - sn[i] * p[i].y, sn[i] * p[i].x + cs[i] * p[i].y);
+            x = Piece<T>::store(p);
+        }
+        *reinterpret_cast<uint4 *>(dst) = x;
+    }
+}
+
+} // namespace
+} // namespace vkb
+
+extern "C" vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged_kv *kv, const void *q,
+                                                   uint64_t q_stride, const void *k, uint64_t k_stride, const void *v,
+                                                   uint64_t v_stride, const uint32_t *positions, const uint32_t *slots,
+                                                   uint32_t n_tokens, uint32_t heads, float rope_base, void *q_out,
+                                                   uint64_t q_out_stride, uint32_t *status, void *stream)
+{
+    using namespace vkb;
+    _CHECK_ARGS(kv_fits(kv));
+    _CHECK_ARGS(heads > 0 && heads <= 65535 && heads % kv->kv_heads == 0);
+    const uint32_t es = paged_elem_bytes(kv->dtype), hd = kv->head_dim;
+    _CHECK_ARGS(rope_base <= 0.f || (rope_base > 1.f && std::isfinite(rope_base)));
+    if (n_tokens == 0)
+        return VKLLM_ERR_OK;
+    _CHECK_ARGS(n_tokens <= 0x7fffffffu);
+    _CHECK_ARGS(rows_fit(q, q_stride, (uint64_t)heads * hd, es) && rows_fit(q_out, q_out_stride, (uint64_t)heads * hd, es));
+    _CHECK_ARGS(rows_fit(k, k_stride, (uint64_t)kv->kv_heads * hd, es) &&
+                rows_fit(v, v_stride, (uint64_t)kv->kv_heads * hd, es));
+    _CHECK_ARGS(q != q_out || q_stride == q_out_stride);
+    _CHECK_ARGS(words(positions) && words(slots) && words(status));
+    int sms = 0;
+    _CHECK(check_device(kv->k, &sms, nullptr));
+    RopeArgs a;
+    a.kv = *kv;
+    a.q = q, a.k = k, a.v = v, a.q_out = q_out;
+    a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.q_out_stride = q_out_stride;
+    a.positions = positions, a.slots = slots, a.n_tokens = n_tokens, a.heads = heads, a.status = status;
+    // one power, then products: each costs half a unit in the 64th bit, 2^-57 of a frequency at the last
+    const long double base = rope_base <= 0.f ? 10000.0L : (long double)rope_base;
+    const long double ratio = powl(base, -2.0L / hd);
+    long double f = 0x1p64L / (2.0L * 3.14159265358979323846264338327950288L);
+    for (uint32_t w = 0; w < hd / 2; ++w, f *= ratio)
+        a.turns[w] = (uint64_t)f;
+    const uint32_t pieces = hd * es / 16, threads = kRopeThreads / pieces * pieces, lanes = threads / pieces;
+    // few tokens: several blocks share a token's rows so that the call reaches about two blocks an SM
+    const uint32_t passes = (heads + 2 * kv->kv_heads + lanes - 1) / lanes;
+    uint32_t shares = 1;
+    while (shares < passes && (uint64_t)n_tokens * shares < 2u * (uint32_t)sms)
+        ++shares;
+    const dim3 grid(n_tokens, shares);
+    if (kv->dtype == vkllm_dtype_float16)
+        k_paged_rope_write<__half><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
+    else
+        k_paged_rope_write<float><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
+    VKB_CUDA(cudaGetLastError());
+    return VKLLM_ERR_OK;
+}

@@ -4,6 +4,7 @@
 
 #include "internal.h"
 #include "vkllm_b200.h"
+#include "vkllm_b200_paged.h"
 #include "vkllm_kvcache.h"
 #include "vkllm_models_llama2.h"
 
@@ -86,6 +87,12 @@ extern "C" size_t vkllm_b200_sizeof(const char *name)
         return sizeof(vkllm_kvcache);
     if (!strcmp(name, "block_weights"))
         return sizeof(block_weights);
+    if (!strcmp(name, "vkllm_b200_paged_table"))
+        return sizeof(vkllm_b200_paged_table);
+    if (!strcmp(name, "vkllm_b200_paged_kv"))
+        return sizeof(vkllm_b200_paged_kv);
+    if (!strcmp(name, "vkllm_b200_logit_rules"))
+        return sizeof(vkllm_b200_logit_rules);
     return 0;
 }
 

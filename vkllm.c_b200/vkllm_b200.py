@@ -87,12 +87,37 @@ class Llama2Config(C.Structure):
                 ("rope_freq_base", C.c_float), ("rms_eps", C.c_float), ("init_std", C.c_float)]
 
 
+class PagedTable(C.Structure):
+    """struct vkllm_b200_paged_table (include/vkllm_b200_paged.h); pointers are device addresses."""
+    _fields_ = [("table", C.c_void_p), ("free_pages", C.c_void_p), ("stride", C.c_uint64), ("n_seqs", C.c_uint32),
+                ("cols", C.c_uint32), ("page_rows", C.c_uint32), ("n_pages", C.c_uint32)]
+
+
+class PagedKV(C.Structure):
+    """struct vkllm_b200_paged_kv; strides in elements."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_uint64), ("head_stride", C.c_uint64),
+                ("row_stride", C.c_uint64), ("n_pages", C.c_uint32), ("page_rows", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("dtype", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class LogitRules(C.Structure):
+    """struct vkllm_b200_logit_rules; a None pointer turns its rule off."""
+    _fields_ = [(n, C.c_void_p) for n in
+                ("history", "prompt_lens", "history_lens", "repetition", "frequency", "presence", "bias_starts",
+                 "bias_ids", "bias_values", "mask")] + [("history_stride", C.c_uint64), ("mask_stride", C.c_uint64)]
+
+
 class TokenIdArray(C.Structure):
     _fields_ = [("alloc_n", C.c_size_t), ("used_n", C.c_size_t), ("data", C.POINTER(C.c_uint32))]
 
 
 PT = C.POINTER(Tensor)
 _lib = None
+
+# include/vkllm_b200_paged.h
+NO_SLOT = 0xffffffff
+PAGED_BAD_PAGE, PAGED_TOO_LONG, PAGED_NO_PAGES, PAGED_TOO_MANY, PAGED_BAD_SLOT = 1, 2, 4, 8, 16
+PAGED_WORKSPACE_BYTES = 16 << 20
 
 # name -> (restype, argtypes)
 _SIGS = {
@@ -198,6 +223,19 @@ _SIGS = {
                                                  C.POINTER(C.c_float), C.POINTER(C.c_uint64)]),
     "vkllm_b200_attention_decode_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32,
                                                       C.c_uint32, C.c_uint32, C.c_float, C.c_void_p, C.c_void_p]),
+    # the paged serving operators: structs by address (C.byref, or a buffer with the same bytes), arrays as
+    # device addresses
+    "vkllm_b200_paged_check": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p]),
+    "vkllm_b200_paged_append": (C.c_int, [C.c_void_p] * 9 + [C.c_uint32, C.c_void_p, C.c_void_p]),
+    "vkllm_b200_paged_release": (C.c_int, [C.c_void_p] * 8),
+    "vkllm_b200_paged_rope_write": (C.c_int, [C.c_void_p] + [C.c_void_p, C.c_uint64] * 3 +
+                                    [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_float, C.c_void_p, C.c_uint64,
+                                     C.c_void_p, C.c_void_p]),
+    "vkllm_b200_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p,
+                                             C.c_float, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p,
+                                             C.c_void_p]),
+    "vkllm_b200_logits_apply": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32,
+                                          C.c_void_p, C.c_uint64, C.c_void_p]),
     "vkllm_b200_sizeof": (C.c_size_t, [C.c_char_p]),
     "vkllm_b200_offsetof": (C.c_size_t, [C.c_char_p, C.c_char_p]),
 }
