@@ -2,9 +2,30 @@
 //
 //   out = sum_j exp(scale q . k_j - m) v_j / sum_j exp(scale q . k_j - m),  j < len,  m = max_j scale q . k_j
 //
-// One pass over the keys with a running maximum and sum, in fp32. A block takes one query head of one
-// sequence; its warps take the keys in turn and join at the end.
-#include <cfloat>
+// Every cached row is read once for all the query heads that share its key head: 2 to 32 flops a byte,
+// so HBM bounds the call, and what matters is that every SM keeps enough loads in flight from the
+// first microsecond to the last.
+//
+// Work. Lengths are known on the device only, so the kernel divides the work itself. An item is one
+// (sequence, key head, tile of up to 8 or 16 of its queries); its keys are cut into tiles of 4 slices,
+// one slice per warp (16 keys in fp16, 8 in fp32). All tiles of all items form one line, of which every CTA
+// of a grid that fills the GPU takes an equal part: a long sequence spreads over all SMs and short ones
+// share a CTA. A CTA that holds only a part of an item leaves (m, l, O) in the workspace and counts
+// itself at the item; the last one to arrive joins the parts in the order of the line, so the result
+// does not depend on who was last.
+//
+// Loads. Each warp streams its own slices through a private ring of cp.async stages, also across the
+// borders of items: no barrier of the CTA stands between a load and its use. Page ids are read one tile ahead of
+// the rows that they lead to. Rows past the end, and rows of bad pages, are filled with zeros without being read and masked out of the scores.
+//
+// fp16: S^T = K Q^T on the tensor cores (mma.sync m16n8k16: 16 keys x 8 queries), so that the 8 columns
+// take up to 8 queries that share the keys and each lane keeps the statistics of two of them; then O^T += V^T P with
+// P^T moved into operand order by movmatrix. The weights are kept as the sum of two fp16 parts, scaled by
+// 2^15: one part alone would double the error of the rounded output, and unscaled ones would lose their bits
+// below fp16's range where one key outweighs very many small ones (the tensor cores have the time: they idle behind the loads).
+// fp32: plain FMAs; 4 lanes share a key's dot product, and every lane owns head_dim / 32 of the output.
+#include <atomic>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "../runtime/internal.h"
@@ -14,86 +35,762 @@ namespace vkb
 namespace
 {
 
-constexpr uint32_t kAttThreads = 256;
+constexpr uint32_t kWarps = 4, kThreads = kWarps * 32;
+constexpr uint32_t kCounters = 1024;      // words at the start of the workspace, one per CTA of the grid
+constexpr uint32_t kMinTiles = 4;         // least tiles of a CTA (see launch)
+constexpr float kWeightShift = 15.f;      // weights are at most 2^15, below fp16's 65504
 
 struct PagedAttArgs
 {
     vkllm_b200_paged_kv kv;
-    vkllm_b200_paged_table t;
+    const uint32_t *table;
+    uint64_t table_stride;
+    uint32_t n_seqs;
+    uint32_t cap; // most rows of a sequence (cols * page_rows)
     const void *q;
     void *out;
     uint64_t q_stride, out_stride;
     const uint32_t *lens;
-    uint32_t heads;
-    float scale;
+    uint32_t group;  // queries that share a key head
+    uint32_t qtiles; // tiles of these queries
+    uint32_t gq;     // queries of a tile (the last tile may have fewer)
+    float scale_log2; // scale * log2(e): the softmax runs in powers of two
     uint32_t *status;
+    uint32_t *counters;
+    float *parts; // [2 * grid] parts of items: [gq][HP] O, then [gq] m, [gq] l
+    uint32_t part_stride;
 };
 
-template <typename T> __global__ void __launch_bounds__(kAttThreads) k_paged_attention(const PagedAttArgs a)
+template <typename T, int HP> struct Shape
 {
-    __shared__ float acc_sm[kAttThreads / 32][256], m_sm[kAttThreads / 32], l_sm[kAttThreads / 32];
-    const uint32_t h = blockIdx.x, s = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t hd = a.kv.head_dim, R = a.kv.page_rows, kh = h / (a.heads / a.kv.kv_heads);
-    const uint64_t cap = table_rows(a.t);
-    uint32_t len = a.lens[s], e = 0;
-    if (len > cap)
-        len = (uint32_t)cap, e = VKLLM_B200_PAGED_TOO_LONG;
-    float q[8], acc[8], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
+    static constexpr uint32_t kKeys = sizeof(T) == 2 ? 16 : 8;                  // keys of a slice
+    static constexpr uint32_t kRow = HP * sizeof(T);                            // bytes of a row in shared memory
+    static constexpr uint32_t kStage = 2 * kKeys * kRow;                        // K and V of a slice
+    static constexpr uint32_t kQBytes = sizeof(T) == 4 ? 8 * HP * 4 : 0;        // the queries (fp32 only)
+    static constexpr uint32_t kStages = HP == 64 ? 6 : (HP == 256 && sizeof(T) == 4) ? 2 : 3;
+    static constexpr uint32_t kPitch = HP + 4;                                  // floats of a row of the join buffer
+    static constexpr uint32_t kRing = kWarps * kStages * kStage;
+    static constexpr uint32_t kSmem = kRing + kQBytes + kWarps * 8 * kPitch * 4 + kWarps * 8 * 2 * 4 + kWarps * kStages * 4;
+    static constexpr uint32_t kCtas = HP == 256 ? 1 : 2; // per SM
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit()
+{
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N> __device__ __forceinline__ void cp_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float pow2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t v)
+{
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+// exp2's base for a maximum: any finite number does where no key counts yet.
+__device__ __forceinline__ float finite_base(float m)
+{
+    return m == -INFINITY ? 0.f : m;
+}
+
+// A place in the line of tiles: tile `tile` of `tiles` of item (seq, hq), hq = key head * qtiles + query tile.
+struct Cursor
+{
+    uint32_t seq, hq, tile, tiles, len;
+
+    __device__ __forceinline__ void set_len(const PagedAttArgs &a, uint32_t tile_keys)
     {
-        const uint32_t d = lane + 32 * i;
-        q[i] = d < hd ? to_f32<T>(((const T *)a.q)[s * a.q_stride + (uint64_t)h * hd + d]) : 0.f;
-        acc[i] = 0.f;
+        len = min(a.lens[seq], a.cap);
+        tiles = (len + tile_keys - 1) / tile_keys;
     }
-    for (uint32_t j = warp; j < len; j += kAttThreads / 32)
+    // One tile on; stays at the last item's end when there is no further one.
+    __device__ __forceinline__ void next(const PagedAttArgs &a, uint32_t items, uint32_t tile_keys)
     {
-        const uint32_t page = a.t.table[s * a.t.stride + j / R];
-        if (page >= a.t.n_pages)
+        if (++tile < tiles)
+            return;
+        tile = 0;
+        if (++hq < items)
+            return;
+        hq = 0;
+        do
+            ++seq;
+        while (seq < a.n_seqs && (set_len(a, tile_keys), tiles == 0));
+    }
+};
+
+// The stream of one warp's slices: page ids one tile ahead, rows kStages - 1 tiles ahead.
+template <typename T, int HP, bool EXACT> struct Loader
+{
+    using S = Shape<T, HP>;
+    static constexpr uint32_t kPieces = S::kRow / 16;
+    Cursor c;
+    uint32_t left; // tiles still to load
+    uint32_t page; // of key `lane % kKeys` of the slice at c
+    uint32_t ring; // shared address of the warp's ring
+    uint32_t *valid; // [kStages] masks of the slice's keys that count
+    uint32_t stage = 0, status = 0;
+
+    __device__ __forceinline__ uint32_t key(uint32_t warp, uint32_t lane) const
+    {
+        return (c.tile * kWarps + warp) * S::kKeys + lane % S::kKeys;
+    }
+    __device__ __forceinline__ void lookup(const PagedAttArgs &a, uint32_t warp, uint32_t lane)
+    {
+        const uint32_t k = key(warp, lane);
+        page = left && k < c.len ? __ldg(a.table + c.seq * a.table_stride + k / a.kv.page_rows) : 0xffffffffu;
+    }
+    // Issues the slice at c as one group of copies (an empty one behind the end) and moves on.
+    __device__ __forceinline__ void issue(const PagedAttArgs &a, uint32_t items, uint32_t warp, uint32_t lane)
+    {
+        if (left)
         {
-            e |= VKLLM_B200_PAGED_BAD_PAGE;
-            continue;
+            const uint32_t k = key(warp, lane);
+            bool ok = k < c.len;
+            if (ok && page >= a.kv.n_pages)
+                ok = false, status |= VKLLM_B200_PAGED_BAD_PAGE;
+            const uint64_t at = ok ? page * a.kv.page_stride + (c.hq / a.qtiles) * a.kv.head_stride +
+                                         (k % a.kv.page_rows) * a.kv.row_stride
+                                   : 0;
+            const uint32_t mask = __ballot_sync(0xffffffffu, ok) & ((1u << S::kKeys) - 1);
+            if (lane == 0)
+                valid[stage] = mask;
+            if (mask)
+            {
+                const uint32_t base = ring + stage * S::kStage;
+                const uint32_t pieces = EXACT ? kPieces : a.kv.head_dim * (uint32_t)sizeof(T) / 16;
+                uint32_t row = lane / pieces, p = lane % pieces;
+                const uint32_t drow = 32 / pieces, dp = 32 % pieces;
+                constexpr uint32_t kMost = S::kKeys * kPieces / 32;
+#pragma unroll
+                for (uint32_t i = 0; i < kMost; ++i)
+                {
+                    const uint32_t r = row % S::kKeys; // row < kKeys for every copy that is made
+                    const uint64_t off = __shfl_sync(0xffffffffu, at, r) + p * (16 / sizeof(T));
+                    const uint32_t bytes = (mask >> r) & 1u ? 16u : 0u;
+                    if (EXACT || row < S::kKeys)
+                    {
+                        const uint32_t dst = base + r * S::kRow + ((p ^ (r & 7)) * 16);
+                        cp_async16(dst, (const T *)a.kv.k + off, bytes);
+                        cp_async16(dst + S::kKeys * S::kRow, (const T *)a.kv.v + off, bytes);
+                    }
+                    row += drow, p += dp;
+                    if ((!EXACT || kPieces > 32) && p >= pieces)
+                        p -= pieces, ++row;
+                }
+            }
+            --left;
+            c.next(a, items, kWarps * S::kKeys);
+            lookup(a, warp, lane);
         }
-        const uint64_t at = page * a.kv.page_stride + kh * a.kv.head_stride + (j % R) * a.kv.row_stride;
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < hd)
-                dot = fmaf(q[i], to_f32<T>(((const T *)a.kv.k)[at + lane + 32 * i]), dot);
-        dot = warp_sum(dot) * a.scale;
-        const float mn = fmaxf(m, dot), base = mn == -INFINITY ? 0.f : mn;
-        const float p = expf(dot - base), f = expf(m - base);
-        m = mn;
-        l = l * f + p;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < hd)
-                acc[i] = fmaf(p, to_f32<T>(((const T *)a.kv.v)[at + lane + 32 * i]), acc[i] * f);
+        cp_commit();
+        stage = stage + 1 == S::kStages ? 0 : stage + 1;
     }
-    if (e && lane == 0)
-        atomicOr(a.status, e);
+};
+
+// What a warp keeps of an item: statistics and outputs of its keys, for 8 NQ queries.
+template <int HP, int NQ, bool EXACT> struct HalfCore
+{
+    using T = __half;
+    using S = Shape<T, HP>;
+    static constexpr int kK = HP / 16;
+    uint32_t qf[NQ][kK][2]; // Q^T as the B operand
+    float o[NQ][kK][4], m[NQ][2], l[NQ][2];
+
+    __device__ __forceinline__ void start(const PagedAttArgs &a, uint32_t seq, uint32_t head0, uint32_t nq, uint32_t lane,
+                                          float *)
+    {
+        const uint32_t hd = a.kv.head_dim;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        acc_sm[warp][lane + 32 * i] = acc[i];
-    if (lane == 0)
-        m_sm[warp] = m, l_sm[warp] = l;
+        for (int n = 0; n < NQ; ++n)
+        {
+            const uint32_t qi = n * 8 + (lane >> 2);
+            const T *row = (const T *)a.q + seq * a.q_stride + (uint64_t)(head0 + qi) * hd;
+#pragma unroll
+            for (int k = 0; k < kK; ++k)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                {
+                    const uint32_t d = k * 16 + b * 8 + (lane & 3) * 2;
+                    qf[n][k][b] = qi < nq && (EXACT || d < hd) ? __ldg(reinterpret_cast<const uint32_t *>(row + d)) : 0u;
+                }
+#pragma unroll
+            for (int k = 0; k < kK; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    o[n][k][i] = 0.f;
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+        }
+    }
+
+    __device__ __forceinline__ void slice(const PagedAttArgs &a, uint32_t base, uint32_t mask, uint32_t lane,
+                                          const float *)
+    {
+        float s[NQ][2][4]; // two chains of products
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s[n][0][i] = s[n][1][i] = 0.f;
+        const uint32_t kr = lane & 15;
+#pragma unroll
+        for (int k = 0; k < kK; ++k)
+        {
+            uint32_t f[4];
+            ldsm4(f, base + kr * S::kRow + (((2 * k + (lane >> 4)) ^ (kr & 7)) * 16));
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+                mma16816(s[n][k & 1], f, qf[n][k][0], qf[n][k][1]);
+        }
+        const bool in0 = (mask >> (lane >> 2)) & 1u, in1 = (mask >> ((lane >> 2) + 8)) & 1u;
+        uint32_t hi[NQ][2], lo[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+        {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x[i] = (i < 2 ? in0 : in1) ? (s[n][0][i] + s[n][1][i]) * a.scale_log2 : -INFINITY;
+            float f[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+            {
+                float mx = fmaxf(x[i], x[i + 2]);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                mx = fmaxf(mx, m[n][i]);
+                const float b = finite_base(mx);
+                f[i] = pow2(m[n][i] - b);
+                m[n][i] = mx;
+                x[i] = pow2(x[i] - b + kWeightShift);
+                x[i + 2] = pow2(x[i + 2] - b + kWeightShift);
+                l[n][i] = fmaf(l[n][i], f[i], x[i] + x[i + 2]);
+            }
+            if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f))
+#pragma unroll
+                for (int k = 0; k < kK; ++k)
+                {
+                    o[n][k][0] *= f[0], o[n][k][1] *= f[1];
+                    o[n][k][2] *= f[0], o[n][k][3] *= f[1];
+                }
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+            {
+                const uint32_t h = pack2(x[2 * b], x[2 * b + 1]);
+                const float2 hf = unpack2(h);
+                hi[n][b] = transpose8x8(h);
+                lo[n][b] = transpose8x8(pack2(x[2 * b] - hf.x, x[2 * b + 1] - hf.y));
+            }
+        }
+        const uint32_t vr = (lane & 7) + ((lane >> 4) & 1) * 8, vbase = base + S::kKeys * S::kRow + vr * S::kRow;
+#pragma unroll
+        for (int k = 0; k < kK; ++k)
+        {
+            uint32_t f[4];
+            ldsm4_t(f, vbase + (((2 * k + ((lane >> 3) & 1)) ^ (vr & 7)) * 16));
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+            {
+                mma16816(o[n][k], f, hi[n][0], hi[n][1]);
+                mma16816(o[n][k], f, lo[n][0], lo[n][1]);
+            }
+        }
+    }
+
+    // Queries 8 n .. 8 n + 7 into the join buffer: os [8][kPitch], ml [8][2].
+    __device__ __forceinline__ void deposit(int n, float *os, float *ml, uint32_t lane)
+    {
+#pragma unroll
+        for (int nn = 0; nn < NQ; ++nn)
+            if (nn == n)
+            {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                {
+                    const uint32_t q = (lane & 3) * 2 + i;
+                    float t = l[nn][i];
+                    t += __shfl_xor_sync(0xffffffffu, t, 4);
+                    t += __shfl_xor_sync(0xffffffffu, t, 8);
+                    t += __shfl_xor_sync(0xffffffffu, t, 16);
+                    if (lane < 4)
+                        ml[q * 2] = m[nn][i], ml[q * 2 + 1] = t;
+#pragma unroll
+                    for (int k = 0; k < kK; ++k)
+                    {
+                        os[q * S::kPitch + k * 16 + (lane >> 2)] = o[nn][k][i];
+                        os[q * S::kPitch + k * 16 + (lane >> 2) + 8] = o[nn][k][i + 2];
+                    }
+                }
+            }
+    }
+};
+
+// fp32: 8 keys of a slice; lane = (part << 3) | key computes a quarter of that key's dot products (the
+// 16-byte pieces p with p % 4 == part); for the outputs a lane owns the pieces lane % kP, lane % kP + 32 ...
+template <int HP, bool EXACT> struct FloatCore
+{
+    using T = float;
+    using S = Shape<T, HP>;
+    static constexpr int kP = HP / 4;                       // pieces of a row
+    static constexpr int kOwn = kP > 32 ? kP / 32 : 1;      // pieces that a lane owns
+    static constexpr int kHalves = kP < 32 ? 32 / kP : 1;   // lane groups that share the keys (HP = 64: 2)
+    float4 o[8][kOwn];
+    float m[8], l[8];
+    uint32_t nq;
+
+    __device__ __forceinline__ void start(const PagedAttArgs &a, uint32_t seq, uint32_t head0, uint32_t n, uint32_t lane,
+                                          float *qs)
+    {
+        // the CTA's warps are at the same item here: each loads two of its queries
+        const uint32_t hd = a.kv.head_dim, warp = threadIdx.x >> 5;
+        nq = n;
+        for (uint32_t i = warp; i < 8; i += kWarps)
+            for (uint32_t d = lane; d < HP; d += 32)
+                qs[i * HP + d] = i < n && d < hd ? ((const T *)a.q)[seq * a.q_stride + (uint64_t)(head0 + i) * hd + d] : 0.f;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+#pragma unroll
+            for (int k = 0; k < kOwn; ++k)
+                o[i][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            m[i] = -INFINITY, l[i] = 0.f;
+        }
+    }
+
+    __device__ __forceinline__ void slice(const PagedAttArgs &a, uint32_t base, uint32_t mask, uint32_t lane,
+                                          const float *qs)
+    {
+        extern __shared__ __align__(128) unsigned char sm[];
+        const uint32_t off = base - (uint32_t)__cvta_generic_to_shared(sm);
+        const float4 *K = reinterpret_cast<const float4 *>(sm + off);
+        const float4 *V = K + S::kKeys * kP;
+        const uint32_t key = lane & 7, part = lane >> 3;
+        float4 kr[kP / 4];
+#pragma unroll
+        for (int j = 0; j < kP / 4; ++j)
+            kr[j] = K[key * kP + ((4 * j + part) ^ key)];
+        const bool in = (mask >> key) & 1u;
+        float p[8], f[8];
+        bool moved = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            if (i >= nq)
+                break;
+            float d = 0.f;
+#pragma unroll
+            for (int j = 0; j < kP / 4; ++j)
+            {
+                const float4 q = reinterpret_cast<const float4 *>(qs + i * HP)[4 * j + part];
+                d = fmaf(q.x, kr[j].x, d), d = fmaf(q.y, kr[j].y, d);
+                d = fmaf(q.z, kr[j].z, d), d = fmaf(q.w, kr[j].w, d);
+            }
+            d += __shfl_xor_sync(0xffffffffu, d, 8);
+            d += __shfl_xor_sync(0xffffffffu, d, 16);
+            const float x = in ? d * a.scale_log2 : -INFINITY;
+            float mx = x;
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, m[i]);
+            const float b = finite_base(mx);
+            f[i] = pow2(m[i] - b);
+            moved |= f[i] != 1.f;
+            m[i] = mx;
+            p[i] = pow2(x - b);
+            l[i] = fmaf(l[i], f[i], p[i]);
+        }
+        if (__any_sync(0xffffffffu, moved))
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                if (i >= nq)
+                    break;
+#pragma unroll
+                for (int k = 0; k < kOwn; ++k)
+                    o[i][k].x *= f[i], o[i][k].y *= f[i], o[i][k].z *= f[i], o[i][k].w *= f[i];
+            }
+        const uint32_t own = lane % kP, first = kHalves > 1 ? lane / kP : 0;
+#pragma unroll
+        for (uint32_t j = 0; j < S::kKeys / kHalves; ++j)
+        {
+            const uint32_t r = j * kHalves + first;
+            float4 v[kOwn];
+#pragma unroll
+            for (int k = 0; k < kOwn; ++k)
+                v[k] = V[r * kP + ((own + 32 * k) ^ (r & 7))];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                if (i >= nq)
+                    break;
+                const float w = __shfl_sync(0xffffffffu, p[i], r);
+#pragma unroll
+                for (int k = 0; k < kOwn; ++k)
+                {
+                    o[i][k].x = fmaf(w, v[k].x, o[i][k].x), o[i][k].y = fmaf(w, v[k].y, o[i][k].y);
+                    o[i][k].z = fmaf(w, v[k].z, o[i][k].z), o[i][k].w = fmaf(w, v[k].w, o[i][k].w);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void deposit(int, float *os, float *ml, uint32_t lane)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            float t = l[i];
+            t += __shfl_xor_sync(0xffffffffu, t, 1);
+            t += __shfl_xor_sync(0xffffffffu, t, 2);
+            t += __shfl_xor_sync(0xffffffffu, t, 4);
+            if (lane == 0)
+                ml[i * 2] = m[i], ml[i * 2 + 1] = t;
+#pragma unroll
+            for (int k = 0; k < kOwn; ++k)
+            {
+                float4 v = o[i][k];
+                if (kHalves > 1)
+                {
+                    v.x += __shfl_xor_sync(0xffffffffu, v.x, 16), v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+                    v.z += __shfl_xor_sync(0xffffffffu, v.z, 16), v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+                }
+                if (kHalves == 1 || lane < kP)
+                    *reinterpret_cast<float4 *>(os + i * S::kPitch + 4 * (lane % kP + 32 * k)) = v;
+            }
+        }
+    }
+};
+
+// The queries of the join buffer, joined over its warps: `gq` queries from query q0 of the item, to the output or to a part.
+template <typename T, int HP>
+__device__ __forceinline__ void join_warps(const PagedAttArgs &a, const float *os, const float *ml, uint32_t gq,
+                                           uint32_t q0, uint32_t seq, uint32_t head0, float *part, uint32_t part_q)
+{
+    using S = Shape<T, HP>;
+    const uint32_t hd = a.kv.head_dim;
+    for (uint32_t i = threadIdx.x; i < gq * (HP / 4); i += kThreads)
+    {
+        const uint32_t q = i / (HP / 4), d = i % (HP / 4) * 4;
+        float mx = -INFINITY;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w)
+            mx = fmaxf(mx, ml[(w * 8 + q) * 2]);
+        const float b = finite_base(mx);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w)
+        {
+            const float f = pow2(ml[(w * 8 + q) * 2] - b);
+            const float4 v = *reinterpret_cast<const float4 *>(os + (w * 8 + q) * S::kPitch + d);
+            l = fmaf(f, ml[(w * 8 + q) * 2 + 1], l);
+            o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+        }
+        if (part)
+        {
+            *reinterpret_cast<float4 *>(part + (q0 + q) * HP + d) = o;
+            if (d == 0)
+                part[part_q * HP + q0 + q] = mx, part[part_q * (HP + 1) + q0 + q] = l;
+        }
+        else if (d < hd)
+        {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            T *dst = (T *)a.out + seq * a.out_stride + (uint64_t)(head0 + q0 + q) * hd + d;
+            if constexpr (sizeof(T) == 2)
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
+            else
+                *reinterpret_cast<float4 *>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        }
+    }
+}
+
+template <typename Core, typename T, int HP, int NQ, bool EXACT>
+__global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attention(const PagedAttArgs a)
+{
+    using S = Shape<T, HP>;
+    constexpr uint32_t kTile = kWarps * S::kKeys;
+    extern __shared__ __align__(128) unsigned char sm[];
+    float *qs = reinterpret_cast<float *>(sm + S::kRing);
+    float *os = reinterpret_cast<float *>(sm + S::kRing + S::kQBytes); // [kWarps][8][kPitch]
+    float *ml = os + kWarps * 8 * S::kPitch;                           // [kWarps][8][2]
+    uint32_t *valid = reinterpret_cast<uint32_t *>(ml + kWarps * 8 * 2); // [kWarps][kStages]
+    __shared__ uint64_t sums[kWarps];
+    __shared__ Cursor first;
+    __shared__ uint32_t last_one;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.kv.head_dim;
+    const uint32_t items = a.kv.kv_heads * a.qtiles; // of a sequence
+    if (!EXACT) // the pieces behind head_dim are never loaded: they have to be zeros, not whatever was there
+        for (uint32_t i = tid; i < S::kRing / 16; i += kThreads)
+            reinterpret_cast<uint4 *>(sm)[i] = make_uint4(0, 0, 0, 0);
+
+    // This CTA's part of the line: every thread sums a run of sequences, the one in whose run the part
+    // begins finds its place. On the way, sequences without keys get their zeros (each from one CTA).
+    const uint32_t per_thread = (a.n_seqs + kThreads - 1) / kThreads;
+    uint64_t mine = 0;
+    uint32_t status = 0;
+    for (uint32_t i = 0; i < per_thread; ++i)
+    {
+        const uint32_t s = tid * per_thread + i;
+        const uint32_t len = s < a.n_seqs ? a.lens[s] : 1;
+        if (s < a.n_seqs)
+        {
+            if (len > a.cap)
+                status = VKLLM_B200_PAGED_TOO_LONG;
+            mine += (min(len, a.cap) + kTile - 1) / kTile;
+        }
+        uint32_t empty = __ballot_sync(0xffffffffu, len == 0 && s % gridDim.x == blockIdx.x);
+        while (empty)
+        {
+            const uint32_t z = __shfl_sync(0xffffffffu, s, __ffs(empty) - 1);
+            empty &= empty - 1;
+            uint4 *row = reinterpret_cast<uint4 *>((T *)a.out + z * a.out_stride);
+            for (uint32_t d = lane; d < a.kv.kv_heads * a.group * hd * sizeof(T) / 16; d += 32)
+                row[d] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    uint64_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+    {
+        const uint64_t t = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o)
+            before += t;
+    }
+    if (lane == 31)
+        sums[warp] = before;
     __syncthreads();
-    float mx = -INFINITY;
-    for (uint32_t w = 0; w < kAttThreads / 32; ++w)
-        mx = fmaxf(mx, m_sm[w]);
-    if (mx == -INFINITY)
-        mx = 0.f;
-    for (uint32_t d = threadIdx.x; d < hd; d += kAttThreads)
+    uint64_t total = 0;
+    before -= mine;
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w)
     {
-        float o = 0.f, sum = 0.f;
-        for (uint32_t w = 0; w < kAttThreads / 32; ++w)
-        {
-            const float f = expf(m_sm[w] - mx);
-            o = fmaf(f, acc_sm[w][d], o);
-            sum = fmaf(f, l_sm[w], sum);
-        }
-        ((T *)a.out)[s * a.out_stride + (uint64_t)h * hd + d] = from_f32<T>(sum == 0.f ? 0.f : o / sum);
+        if (w < warp)
+            before += sums[w];
+        total += sums[w];
     }
+    total *= items;
+    before *= items;
+    mine *= items;
+    const uint64_t share = (total + gridDim.x - 1) / gridDim.x, per = share < kMinTiles ? kMinTiles : share;
+    const uint64_t begin = blockIdx.x * per, end = begin + per < total ? begin + per : total;
+    if (status)
+        atomicOr(a.status, status);
+    if (begin >= total)
+        return;
+    if (before <= begin && begin < before + mine)
+    {
+        Cursor c;
+        c.seq = tid * per_thread;
+        uint64_t at = before;
+        for (; c.seq < a.n_seqs; ++c.seq)
+        {
+            c.set_len(a, kTile);
+            const uint64_t n = (uint64_t)c.tiles * items;
+            if (begin < at + n)
+                break;
+            at += n;
+        }
+        c.hq = (uint32_t)((begin - at) / c.tiles);
+        c.tile = (uint32_t)((begin - at) % c.tiles);
+        first = c;
+    }
+    __syncthreads();
+
+    Cursor c = first;
+    Loader<T, HP, EXACT> ld;
+    ld.c = c;
+    ld.left = (uint32_t)(end - begin);
+    ld.ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * S::kStages * S::kStage;
+    ld.valid = valid + warp * S::kStages;
+    ld.lookup(a, warp, lane);
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < S::kStages; ++i)
+        ld.issue(a, items, warp, lane);
+
+    Core core;
+    uint32_t stage = 0;
+    uint64_t at = begin;
+    while (at < end && c.seq < a.n_seqs) // (the second holds unless lens is written meanwhile)
+    {
+        // one item, or this CTA's part of it
+        const uint32_t tiles = c.tiles, from = c.tile, n = (uint32_t)min((uint64_t)(tiles - from), end - at);
+        const uint32_t qt = c.hq % a.qtiles, head0 = c.hq / a.qtiles * a.group + qt * a.gq;
+        const uint32_t nq = min(a.gq, a.group - qt * a.gq);
+        core.start(a, c.seq, head0, nq, lane, qs);
+        for (uint32_t i = 0; i < n; ++i)
+        {
+            cp_wait<S::kStages - 2>();
+            __syncwarp();
+            ld.issue(a, items, warp, lane); // into the stage that the warp read before
+            const uint32_t mask = ld.valid[stage];
+            if (mask)
+                core.slice(a, ld.ring + stage * S::kStage, mask, lane, qs);
+            stage = stage + 1 == S::kStages ? 0 : stage + 1;
+        }
+        const bool whole = n == tiles;
+        // a part goes to the CTA's first slot when the item began before, else to its second
+        float *part = whole ? nullptr : a.parts + (2 * (uint64_t)blockIdx.x + (from == 0)) * a.part_stride;
+#pragma unroll
+        for (int r = 0; r < NQ; ++r)
+        {
+            if (r * 8 >= nq)
+                break;
+            core.deposit(r, os + warp * 8 * S::kPitch, ml + warp * 8 * 2, lane);
+            __syncthreads();
+            join_warps<T, HP>(a, os, ml, min(nq - r * 8, 8u), r * 8, c.seq, head0, part, a.gq);
+            __syncthreads();
+        }
+        if (!whole)
+        {
+            // CTAs c0 .. c1 hold the item's parts
+            const uint64_t item = at - from;
+            const uint32_t c0 = (uint32_t)(item / per), c1 = (uint32_t)((item + tiles - 1) / per);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0)
+                last_one = atomicAdd(a.counters + c0, 1u) == c1 - c0;
+            __syncthreads();
+            if (last_one)
+            {
+                __threadfence();
+                if (tid == 0)
+                    a.counters[c0] = 0; // ready for the next call
+                for (uint32_t r = 0; r * 8 < nq; ++r)
+                {
+                    // each warp joins every fourth part of 8 queries, then the warps join as above
+                    const uint32_t gq = min(nq - r * 8, 8u);
+                    for (uint32_t q = 0; q < gq; ++q)
+                    {
+                        constexpr int kOwn = HP > 128 ? HP / 128 : 1;
+                        float mx = -INFINITY, l = 0.f;
+                        float4 o[kOwn];
+#pragma unroll
+                        for (int k = 0; k < kOwn; ++k)
+                            o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        const bool lane_on = HP >= 128 || lane < HP / 4;
+#pragma unroll 4
+                        for (uint32_t p = c0 + warp; p <= c1; p += kWarps)
+                        {
+                            const float *src = a.parts + (2 * (uint64_t)p + (p == c0)) * a.part_stride;
+                            const float pm = __ldcg(src + a.gq * HP + r * 8 + q), pl = __ldcg(src + a.gq * (HP + 1) + r * 8 + q);
+                            float4 v[kOwn];
+#pragma unroll
+                            for (int k = 0; k < kOwn; ++k)
+                                v[k] = lane_on ? __ldcg(reinterpret_cast<const float4 *>(src + (r * 8 + q) * HP) + lane + 32 * k)
+                                               : make_float4(0.f, 0.f, 0.f, 0.f);
+                            const float mn = fmaxf(mx, pm), b = finite_base(mn), f = pow2(mx - b), g = pow2(pm - b);
+                            mx = mn;
+                            l = l * f + pl * g;
+#pragma unroll
+                            for (int k = 0; k < kOwn; ++k)
+                            {
+                                o[k].x = o[k].x * f + v[k].x * g, o[k].y = o[k].y * f + v[k].y * g;
+                                o[k].z = o[k].z * f + v[k].z * g, o[k].w = o[k].w * f + v[k].w * g;
+                            }
+                        }
+                        if (lane_on)
+#pragma unroll
+                            for (int k = 0; k < kOwn; ++k)
+                                *reinterpret_cast<float4 *>(os + (warp * 8 + q) * S::kPitch + 4 * (lane + 32 * k)) = o[k];
+                        if (lane == 0)
+                            ml[(warp * 8 + q) * 2] = mx, ml[(warp * 8 + q) * 2 + 1] = l;
+                    }
+                    __syncthreads();
+                    join_warps<T, HP>(a, os, ml, gq, r * 8, c.seq, head0, nullptr, 0);
+                    __syncthreads();
+                }
+            }
+        }
+        at += n;
+        c.tile = from + n - 1;
+        if (at < end)
+            c.next(a, items, kTile);
+    }
+    if (ld.status)
+        atomicOr(a.status, ld.status);
+}
+
+template <typename Core, typename T, int HP, int NQ, bool EXACT>
+vkllm_err_t launch(PagedAttArgs &a, int sms, int device, cudaStream_t s)
+{
+    using S = Shape<T, HP>;
+    auto kernel = k_paged_attention<Core, T, HP, NQ, EXACT>;
+    static std::atomic<bool> done[64]; // the attribute of this kernel, set once a device (twice does no harm)
+    if (device >= 64 || !done[device].load(std::memory_order_relaxed))
+    {
+        VKB_CUDA(cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+        if (device < 64)
+            done[device].store(true, std::memory_order_relaxed);
+    }
+    a.part_stride = a.gq * (HP + 2);
+    a.part_stride = (a.part_stride + 3) / 4 * 4;
+    // most CTAs that can have work, that the counters and the workspace serve, and that the GPU holds at once
+    const uint64_t tiles = (a.cap + (uint64_t)kWarps * S::kKeys - 1) / (kWarps * S::kKeys);
+    const uint64_t work = (tiles * a.n_seqs * a.kv.kv_heads * a.qtiles + kMinTiles - 1) / kMinTiles;
+    const uint64_t room = (VKLLM_B200_PAGED_WORKSPACE_BYTES - kCounters * 4) / (2 * (uint64_t)a.part_stride * 4);
+    uint64_t grid = (uint64_t)sms * S::kCtas;
+    grid = grid < work ? grid : work;
+    grid = grid < room ? grid : room;
+    grid = grid < kCounters ? grid : kCounters;
+    kernel<<<(unsigned)grid, kThreads, S::kSmem, s>>>(a);
+    VKB_CUDA(cudaGetLastError());
+    return VKLLM_ERR_OK;
+}
+
+template <int HP> vkllm_err_t launch_head(PagedAttArgs &a, int sms, int device, cudaStream_t s)
+{
+    const bool exact = a.kv.head_dim == HP;
+    if (a.kv.dtype == vkllm_dtype_float32)
+        return exact ? launch<FloatCore<HP, true>, float, HP, 1, true>(a, sms, device, s)
+                     : launch<FloatCore<HP, false>, float, HP, 1, false>(a, sms, device, s);
+    if (a.gq <= 8)
+        return exact ? launch<HalfCore<HP, 1, true>, __half, HP, 1, true>(a, sms, device, s)
+                     : launch<HalfCore<HP, 1, false>, __half, HP, 1, false>(a, sms, device, s);
+    return exact ? launch<HalfCore<HP, 2, true>, __half, HP, 2, true>(a, sms, device, s)
+                 : launch<HalfCore<HP, 2, false>, __half, HP, 2, false>(a, sms, device, s);
 }
 
 } // namespace
@@ -116,12 +813,23 @@ extern "C" vkllm_err_t vkllm_b200_paged_attention(const struct vkllm_b200_paged_
     _CHECK_ARGS(workspace && aligned_to(workspace, 16) && workspace_bytes >= VKLLM_B200_PAGED_WORKSPACE_BYTES);
     int sms = 0, dev = 0;
     _CHECK(check_device(kv->k, &sms, &dev));
-    const PagedAttArgs a{*kv, *t, q, out, q_stride, out_stride, lens, heads, scale, status};
-    const dim3 grid(heads, t->n_seqs);
-    if (kv->dtype == vkllm_dtype_float16)
-        k_paged_attention<__half><<<grid, kAttThreads, 0, (cudaStream_t)stream>>>(a);
-    else
-        k_paged_attention<float><<<grid, kAttThreads, 0, (cudaStream_t)stream>>>(a);
-    VKB_CUDA(cudaGetLastError());
-    return VKLLM_ERR_OK;
+    PagedAttArgs a;
+    a.kv = *kv;
+    a.table = t->table, a.table_stride = t->stride, a.n_seqs = t->n_seqs;
+    a.cap = (uint32_t)(table_rows(*t) < 0xffffff00ull ? table_rows(*t) : 0xffffff00ull);
+    a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
+    a.lens = lens;
+    a.group = heads / kv->kv_heads;
+    const uint32_t most = kv->dtype == vkllm_dtype_float16 ? 16 : 8; // queries that a CTA takes through one pass
+    a.qtiles = (a.group + most - 1) / most;
+    a.gq = (a.group + a.qtiles - 1) / a.qtiles;
+    a.scale_log2 = scale * 1.44269504088896340736f;
+    a.status = status;
+    a.counters = (uint32_t *)workspace;
+    a.parts = (float *)((char *)workspace + kCounters * 4);
+    if (kv->head_dim <= 64)
+        return launch_head<64>(a, sms, dev, (cudaStream_t)stream);
+    if (kv->head_dim <= 128)
+        return launch_head<128>(a, sms, dev, (cudaStream_t)stream);
+    return launch_head<256>(a, sms, dev, (cudaStream_t)stream);
 }
