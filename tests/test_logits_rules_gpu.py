@@ -106,7 +106,8 @@ def close(got, ref, tol, dtype):
 @pytest.mark.parametrize("on", list(RULES))
 @pytest.mark.parametrize("rows,vocab,past,bias,pad", [(1, 1, 1, 1, 0), (1, 32000, 700, 8, 0), (3, 31, 40, 3, 2),
                                                       (5, 4097, 300, 40, 1), (2, 8192, 5000, 300, 8),
-                                                      (64, 1003, 20, 2, 0), (7, 100003, 900, 33, 3)])
+                                                      (64, 1003, 20, 2, 0), (7, 100003, 900, 33, 3),
+                                                      (3, 20011, 9000, 40, 1), (2, 40, 6144, 0, 0), (2, 9000, 6100, 70, 0)])
 def test_rules(vk, dtype, on, rows, vocab, past, bias, pad):
     import torch
 

@@ -4,11 +4,21 @@
 //   x = x - frequency * (times generated) - (generated ? presence : 0)
 //   x = x + the id's biases;  x = mask bit ? x : -infinity
 //
-// Every logit is read and written once: HBM bounds a large batch, latency a single row. A block takes a
-// piece of the vocabulary of one row, counts the row's history ids that fall into it in shared memory
-// (integer atomics: the order of the additions does not matter) and adds up its biases there, then
-// passes over its logits once. The history (a few KB, in L2) is read once per piece; no table of
-// counts is kept in memory or between calls.
+// Every logit is read and written once (HBM bounds a large batch, latency a single row), but the
+// penalties and biases touch at most as many ids as the history and the lists are long. So two kernels:
+//   k_logits_copy   streams the rows through, with the mask: out = mask bit ? x : -infinity. In place it writes masked
+//                   logits only, and without a mask it is not launched.
+//   k_logits_touch  one block per row: the touched ids with their counts and bias sums in a hash table in
+//                   shared memory, then x read, ruled, rounded once and written at those ids.
+// The second is the first one's programmatic dependent: it builds its tables while the first streams
+// and waits for it only before it touches the rows. The first's grid is resident at once for that
+// reason. (One kernel that counted the history in every piece of a row spent most of its time there:
+// 256 rows of 100003 fp16 logits with 1024 to 2048 ids of history, 62.9 us.)
+// Counts are integer atomics, and biases are added by one warp in the order of the list: the result does
+// not depend on the order of arrival.
+#include <atomic>
+#include <cmath>
+
 #include "paged.cuh"
 #include "../runtime/internal.h"
 
@@ -17,9 +27,16 @@ namespace vkb
 namespace
 {
 
-constexpr uint32_t kRuleThreads = 256;
-constexpr uint32_t kPiece = 4096; // ids per block: 16 KB of counts and 16 KB of biases
-constexpr uint32_t kSeen = 0x80000000u; // in the history at all; the bits below count the times generated
+// 16-byte vectors that a thread has in flight, and CTAs per SM: 48 KB of loads, and registers left for a block of the
+// other kernel. (256 rows of 100003 fp16 logits, all rules: 31.9 us; 4 vectors x 4 or 5 CTAs 33.8, 33.0; two items in
+// flight a thread 34.1.)
+constexpr uint32_t kCopyThreads = 256, kCopyVecs = 2, kCopyCtas = 6;
+constexpr uint32_t kTouchThreads = 512, kHistoryThreads = kTouchThreads - 32; // the last warp sums the biases
+// Slots of the hash table, 16 bytes each; it takes lists of up to 3/4 as many ids (with repeats), longer ones
+// go over ranges of the vocabulary instead. The small table lets more rows share an SM.
+constexpr uint32_t kSlotsSmall = 4096, kSlotsLarge = 8192;
+constexpr uint32_t kNoId = 0xffffffffu; // not an id: vocab < 2^31
+constexpr uint32_t kSeen = 0x80000000u; // in the prompt; the bits below count the times generated
 
 struct RuleArgs
 {
@@ -27,72 +44,316 @@ struct RuleArgs
     const void *x;
     void *y;
     uint64_t x_stride, y_stride;
-    uint32_t vocab;
+    uint32_t vocab, rows;
+    uint32_t slots; // of the hash table, a power of two
+    uint32_t chunk, chunks; // places of a chunk and chunks of a row (the first kernel's)
 };
 
-template <typename T> __global__ void __launch_bounds__(kRuleThreads) k_logits_rules(const RuleArgs a)
+template <typename T> union Vec // 16 bytes of logits
 {
-    __shared__ uint32_t count[kPiece];
-    __shared__ float bias[kPiece];
-    const uint32_t row = blockIdx.y, v0 = blockIdx.x * kPiece, n = min(kPiece, a.vocab - v0), tid = threadIdx.x;
-    for (uint32_t i = tid; i < n; i += kRuleThreads)
-        count[i] = 0, bias[i] = 0.f;
-    __syncthreads();
-    if (a.r.history)
+    uint4 raw;
+    T e[16 / sizeof(T)];
+};
+
+// 4 bits as 4 bytes of 0x00 or 0xff.
+__device__ __forceinline__ uint32_t bytes_of(uint32_t bits)
+{
+    return ((bits & 15u) * 0x00204081u & 0x01010101u) * 0xffu;
+}
+
+// The elements whose bit is set, -infinity for the others.
+template <typename T> __device__ __forceinline__ uint4 masked(uint4 v, uint32_t bits);
+template <> __device__ __forceinline__ uint4 masked<__half>(uint4 v, uint32_t bits)
+{
+    const uint32_t inf = 0xfc00fc00u, lo = bytes_of(bits), hi = bytes_of(bits >> 4);
+    const uint32_t m0 = __byte_perm(lo, 0, 0x1100), m1 = __byte_perm(lo, 0, 0x3322), m2 = __byte_perm(hi, 0, 0x1100),
+                   m3 = __byte_perm(hi, 0, 0x3322);
+    return make_uint4((v.x & m0) | (inf & ~m0), (v.y & m1) | (inf & ~m1), (v.z & m2) | (inf & ~m2), (v.w & m3) | (inf & ~m3));
+}
+template <> __device__ __forceinline__ uint4 masked<float>(uint4 v, uint32_t bits)
+{
+    const uint32_t inf = 0xff800000u;
+    return make_uint4(bits & 1 ? v.x : inf, bits & 2 ? v.y : inf, bits & 4 ? v.z : inf, bits & 8 ? v.w : inf);
+}
+
+// One thread's vectors of a chunk of a row. A row is cut at the 128-byte boundaries of the input, into chunks of
+// equal size: place e of a row is id e - lead, where `lead` elements lie between the boundary at or before the
+// row's start and the row. (Chunks that began at any 16-byte boundary, where warps meet in the middle of lines,
+// copied 51 MB in 24.3 us instead of 21.8.)
+template <typename T> struct CopyItem
+{
+    static constexpr uint32_t E = 16 / sizeof(T), kAll = (1u << E) - 1;
+    const T *x;
+    T *y;
+    const uint32_t *mask;
+    uint32_t lead, end, stop, e0;
+    uint4 v[kCopyVecs];
+    uint32_t allowed[kCopyVecs];
+
+    __device__ __forceinline__ void load(const RuleArgs &a, uint32_t row, uint32_t chunk)
     {
-        const uint32_t have = (uint32_t)min((uint64_t)a.r.history_lens[row], a.r.history_stride);
-        const uint32_t prompt = a.r.prompt_lens ? a.r.prompt_lens[row] : 0;
-        const uint32_t *h = a.r.history + row * a.r.history_stride;
-        for (uint32_t i = tid; i < have; i += kRuleThreads)
+        x = (const T *)a.x + row * a.x_stride;
+        y = (T *)a.y + row * a.y_stride;
+        mask = a.r.mask ? a.r.mask + row * a.r.mask_stride : nullptr;
+        lead = (uint32_t)((uintptr_t)x & 127) / sizeof(T);
+        end = a.vocab + lead;
+        stop = min(end, (chunk + 1) * a.chunk);
+        e0 = chunk * a.chunk + threadIdx.x * E;
+#pragma unroll
+        for (uint32_t k = 0; k < kCopyVecs; ++k)
         {
-            const uint32_t id = h[i] - v0;
-            if (id >= n)
+            const uint32_t e = e0 + k * kCopyThreads * E;
+            allowed[k] = kAll;
+            if (e < lead || e >= stop || e + E > end)
                 continue;
-            if (i >= prompt)
-                atomicAdd(&count[id], 1u);
-            atomicOr(&count[id], kSeen);
-        }
-    }
-    if (a.r.bias_starts && tid < 32)
-    {
-        // one warp, 32 entries at a time: lanes with the same id add one after another, as listed
-        const uint32_t b0 = a.r.bias_starts[row], b1 = a.r.bias_starts[row + 1];
-        for (uint32_t b = b0; b < b1; b += 32)
-        {
-            const bool in = b + tid < b1;
-            const uint32_t id = in ? a.r.bias_ids[b + tid] - v0 : 0xffffffffu;
-            const float value = in ? a.r.bias_values[b + tid] : 0.f;
-            const uint32_t peers = __match_any_sync(0xffffffffu, id);
-            const uint32_t turn = __popc(peers & ((1u << tid) - 1)), turns = __reduce_max_sync(0xffffffffu, turn);
-            for (uint32_t k = 0; k <= turns; ++k)
+            const uint32_t id = e - lead;
+            v[k] = *reinterpret_cast<const uint4 *>(x + id);
+            if (mask)
             {
-                if (turn == k && id < n)
-                    bias[id] += value;
-                __syncwarp();
+                const uint32_t w = id >> 5, last = (id + E - 1) >> 5;
+                const uint32_t lo = __ldg(mask + w), hi = last != w ? __ldg(mask + last) : 0u;
+                allowed[k] &= __funnelshift_r(lo, hi, id & 31);
             }
         }
     }
-    __syncthreads();
+
+    __device__ __forceinline__ void store() const
+    {
+        const bool together = (((uintptr_t)x ^ (uintptr_t)y) & 15) == 0; // the output's 16-byte boundaries are the input's
+#pragma unroll
+        for (uint32_t k = 0; k < kCopyVecs; ++k)
+        {
+            const uint32_t e = e0 + k * kCopyThreads * E;
+            if (e >= stop || e + E <= lead)
+                continue;
+            if (e >= lead && e + E <= end)
+            {
+                if (x == y && allowed[k] == kAll)
+                    continue;
+                Vec<T> o;
+                o.raw = mask ? masked<T>(v[k], allowed[k]) : v[k];
+                if (together)
+                    *reinterpret_cast<uint4 *>(y + (e - lead)) = o.raw;
+                else
+#pragma unroll
+                    for (uint32_t i = 0; i < E; ++i)
+                        y[e - lead + i] = o.e[i];
+                continue;
+            }
+            for (uint32_t i = 0; i < E; ++i) // the row begins or ends inside these 16 bytes
+            {
+                if (e + i < lead || e + i >= end)
+                    continue;
+                const uint32_t id = e + i - lead;
+                y[id] = !mask || ((mask[id >> 5] >> (id & 31)) & 1u) ? x[id] : from_f32<T>(-INFINITY);
+            }
+        }
+    }
+};
+
+template <typename T> __global__ void __launch_bounds__(kCopyThreads) k_logits_copy(const RuleArgs a)
+{
+    asm volatile("griddepcontrol.launch_dependents;");
+    uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const uint32_t rows = gridDim.x / a.chunks, chunks = gridDim.x % a.chunks;
+    while (row < a.rows)
+    {
+        CopyItem<T> item;
+        item.load(a, row, chunk);
+        item.store();
+        row += rows, chunk += chunks;
+        if (chunk >= a.chunks)
+            chunk -= a.chunks, ++row;
+    }
+}
+
+template <typename T> __global__ void __launch_bounds__(kTouchThreads, 4) k_logits_touch(const RuleArgs a)
+{
+    extern __shared__ uint32_t sm[];
+    uint32_t *key = sm, *count = sm + a.slots;
+    float *bias = reinterpret_cast<float *>(sm + 2 * a.slots);
+    uint32_t *list = sm + 3 * a.slots;
+    __shared__ uint32_t listed;
+    const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+    const uint32_t have = a.r.history ? (uint32_t)min((uint64_t)a.r.history_lens[row], a.r.history_stride) : 0;
+    const uint32_t prompt = a.r.history && a.r.prompt_lens ? a.r.prompt_lens[row] : 0;
+    const uint32_t *h = a.r.history + row * a.r.history_stride;
+    const uint32_t b0 = a.r.bias_starts ? a.r.bias_starts[row] : 0, b1 = a.r.bias_starts ? a.r.bias_starts[row + 1] : 0;
+    const uint32_t biases = b1 > b0 ? b1 - b0 : 0;
     const float rep = a.r.repetition ? a.r.repetition[row] : 1.f, freq = a.r.frequency ? a.r.frequency[row] : 0.f,
                 pres = a.r.presence ? a.r.presence[row] : 0.f;
-    const T *x = (const T *)a.x + row * a.x_stride + v0;
-    T *y = (T *)a.y + row * a.y_stride + v0;
-    const uint32_t *mask = a.r.mask ? a.r.mask + row * a.r.mask_stride : nullptr;
-    for (uint32_t i = tid; i < n; i += kRuleThreads)
+    // Few enough ids: hashed, in a table of at least 4/3 their number. Else ranges of the vocabulary one after the
+    // other, each id at its place.
+    const uint64_t ids = (uint64_t)have + biases;
+    const bool hashed = ids <= a.slots / 4 * 3;
+    uint32_t slots = a.slots;
+    if (hashed)
+        while (slots > 64 && slots / 2 >= ids + ids / 3)
+            slots /= 2;
+    bool waited = false;
+    for (uint32_t base = 0; base < (hashed ? 1u : a.vocab); base += a.slots)
     {
-        float v = to_f32<T>(x[i]);
-        const uint32_t c = count[i];
-        if (c)
+        for (uint32_t i = tid; i < slots; i += kTouchThreads)
+            key[i] = kNoId, count[i] = 0, bias[i] = 0.f;
+        __syncthreads();
+        // the slot of an id, or kNoId where it has none
+        auto place = [&](uint32_t id) {
+            if (id >= a.vocab)
+                return kNoId;
+            if (!hashed)
+                return id - base < slots ? id - base : kNoId;
+            uint32_t s = (id * 0x9E3779B1u) >> 8 & (slots - 1);
+            for (;; s = (s + 1) & (slots - 1)) // ends: the table has more slots than ids
+            {
+                uint32_t k = *(volatile uint32_t *)&key[s]; // mostly there already: common ids come often
+                if (k == kNoId)
+                    k = atomicCAS(&key[s], kNoId, id);
+                if (k == kNoId || k == id)
+                    return s;
+            }
+        };
+        if (tid < kHistoryThreads)
         {
-            v = v > 0.f ? v / rep : v * rep;
-            if (c != kSeen)
-                v = v - freq * (float)(c & ~kSeen) - pres;
+            for (uint32_t i0 = tid; i0 < have; i0 += 4 * kHistoryThreads)
+            {
+                uint32_t id[4];
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u)
+                    id[u] = i0 + u * kHistoryThreads < have ? h[i0 + u * kHistoryThreads] : kNoId;
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u)
+                {
+                    const uint32_t s = place(id[u]);
+                    if (s == kNoId)
+                        continue;
+                    if (i0 + u * kHistoryThreads < prompt)
+                        atomicOr(&count[s], kSeen);
+                    else
+                        atomicAdd(&count[s], 1u);
+                }
+            }
         }
-        v += bias[i];
-        if (mask && !((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1u))
-            v = __int_as_float(0xff800000);
-        y[i] = from_f32<T>(v);
+        else
+            // the last warp, 32 entries at a time: lanes with the same id add one after another, as listed
+            for (uint32_t b = 0; b < biases; b += 32)
+            {
+                const bool in = biases - b > lane;
+                const uint32_t id = in ? a.r.bias_ids[b0 + b + lane] : kNoId;
+                const float value = in ? a.r.bias_values[b0 + b + lane] : 0.f;
+                const uint32_t s = place(id), peers = __match_any_sync(0xffffffffu, s);
+                const uint32_t turn = __popc(peers & ((1u << lane) - 1));
+                const uint32_t turns = __reduce_max_sync(0xffffffffu, s == kNoId ? 0u : turn);
+                for (uint32_t k = 0; k <= turns; ++k)
+                {
+                    if (turn == k && s != kNoId)
+                        bias[s] += value;
+                    __syncwarp();
+                }
+                if (biases - b <= 32)
+                    break;
+            }
+        if (tid == 0)
+            listed = 0;
+        __syncthreads();
+        // The touched ids that the mask allows, packed: what is left to do after the wait is one round of loads.
+        const uint32_t *mask = a.r.mask ? a.r.mask + row * a.r.mask_stride : nullptr;
+        for (uint32_t i0 = tid; i0 < slots; i0 += 4 * kTouchThreads)
+        {
+            uint32_t id[4], allowed[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u)
+            {
+                const uint32_t i = i0 + u * kTouchThreads;
+                id[u] = kNoId;
+                if (i < slots && (count[i] != 0 || bias[i] != 0.f))
+                    id[u] = hashed ? key[i] : base + i;
+                allowed[u] = id[u] != kNoId ? (mask ? __ldg(mask + (id[u] >> 5)) : 0xffffffffu) : 0u;
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u)
+                if ((allowed[u] >> (id[u] & 31)) & 1u)
+                    list[atomicAdd(&listed, 1u)] = i0 + u * kTouchThreads;
+        }
+        __syncthreads();
+        if (!waited) // the rows are the first kernel's until it is done
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+        waited = true;
+        // Out of place the logits are read back from the output, where the first kernel just put them: they are in
+        // L2, while the input's lines would be fetched from memory once more.
+        T *y = (T *)a.y + row * a.y_stride;
+        const uint32_t n = listed;
+        for (uint32_t i0 = tid; i0 < n; i0 += 4 * kTouchThreads)
+        {
+            uint32_t id[4], s[4];
+            T x[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u)
+                if (i0 + u * kTouchThreads < n)
+                {
+                    s[u] = list[i0 + u * kTouchThreads];
+                    id[u] = hashed ? key[s[u]] : base + s[u];
+                    x[u] = y[id[u]];
+                }
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u)
+                if (i0 + u * kTouchThreads < n)
+                {
+                    const uint32_t c = count[s[u]];
+                    float v = to_f32<T>(x[u]);
+                    if (c)
+                    {
+                        v = v > 0.f ? v / rep : v * rep;
+                        if (c != kSeen)
+                            v = v - freq * (float)(c & ~kSeen) - pres;
+                    }
+                    y[id[u]] = from_f32<T>(v + bias[s[u]]);
+                }
+        }
+        __syncthreads();
     }
+}
+
+template <typename T> vkllm_err_t launch_rules(RuleArgs &a, int sms, int device, cudaStream_t s)
+{
+    // 16-byte vectors of a row at the worst lead, cut into equal chunks of whole 128-byte lines
+    const uint32_t vecs = (a.vocab + 128 / sizeof(T) - 1 + 16 / sizeof(T) - 1) / (16 / sizeof(T));
+    a.chunks = (vecs + kCopyThreads * kCopyVecs - 1) / (kCopyThreads * kCopyVecs);
+    a.chunk = ((vecs + a.chunks - 1) / a.chunks + 7) / 8 * 8 * (16 / sizeof(T));
+    const bool copy = a.x != a.y || a.r.mask, touch = a.r.history || a.r.bias_starts;
+    static std::atomic<bool> done[64]; // the kernels' attributes, set once a device (twice does no harm)
+    if (device >= 64 || !done[device].load(std::memory_order_relaxed))
+    {
+        VKB_CUDA(cudaFuncSetAttribute((const void *)k_logits_touch<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)(kSlotsLarge * 16)));
+        // an SM changes its split of L1 and shared memory only when it is idle: with the same split for both,
+        // the second kernel's blocks can join the first one's
+        VKB_CUDA(cudaFuncSetAttribute((const void *)k_logits_touch<T>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                      cudaSharedmemCarveoutMaxShared));
+        VKB_CUDA(cudaFuncSetAttribute((const void *)k_logits_copy<T>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                      cudaSharedmemCarveoutMaxShared));
+        if (device < 64)
+            done[device].store(true, std::memory_order_relaxed);
+    }
+    if (copy)
+    {
+        const uint64_t items = (uint64_t)a.rows * a.chunks, most = (uint64_t)sms * kCopyCtas;
+        k_logits_copy<T><<<(unsigned)(items < most ? items : most), kCopyThreads, 0, s>>>(a);
+        VKB_CUDA(cudaGetLastError());
+    }
+    if (!touch)
+        return VKLLM_ERR_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.rows);
+    cfg.blockDim = dim3(kTouchThreads);
+    cfg.dynamicSmemBytes = a.slots * 16;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = copy ? 1 : 0; // alone it follows whatever is in the stream
+    VKB_CUDA(cudaLaunchKernelEx(&cfg, k_logits_touch<T>, a));
+    return VKLLM_ERR_OK;
 }
 
 } // namespace
@@ -105,7 +366,7 @@ extern "C" vkllm_err_t vkllm_b200_logits_apply(const struct vkllm_b200_logit_rul
     using namespace vkb;
     const uint32_t es = paged_elem_bytes(dtype);
     _CHECK_ARGS(rules && es != 0);
-    _CHECK_ARGS(rows > 0 && rows <= 65535 && vocab > 0 && vocab <= 0x7fffffffu);
+    _CHECK_ARGS(rows > 0 && rows <= 65535 && vocab > 0 && vocab <= 0x7fff0000u);
     _CHECK_ARGS(logits && aligned_to(logits, es) && logits_stride >= vocab && logits_stride < (1ull << 40));
     _CHECK_ARGS(out && aligned_to(out, es) && out_stride >= vocab && out_stride < (1ull << 40));
     _CHECK_ARGS(logits != out || logits_stride == out_stride);
@@ -116,13 +377,11 @@ extern "C" vkllm_err_t vkllm_b200_logits_apply(const struct vkllm_b200_logit_rul
     _CHECK_ARGS(!rules->bias_starts || (words(rules->bias_starts) && words(rules->bias_ids) && words(rules->bias_values)));
     _CHECK_ARGS(!rules->mask || (words(rules->mask) && rules->mask_stride >= ((uint64_t)vocab + 31) / 32));
     _CHECK_ARGS(rules->history_stride < (1ull << 40) && rules->mask_stride < (1ull << 40));
-    _CHECK(check_device(logits, nullptr, nullptr));
-    const RuleArgs a{*rules, logits, out, logits_stride, out_stride, vocab};
-    const dim3 grid((vocab + kPiece - 1) / kPiece, rows);
-    if (dtype == vkllm_dtype_float16)
-        k_logits_rules<__half><<<grid, kRuleThreads, 0, (cudaStream_t)stream>>>(a);
-    else
-        k_logits_rules<float><<<grid, kRuleThreads, 0, (cudaStream_t)stream>>>(a);
-    VKB_CUDA(cudaGetLastError());
-    return VKLLM_ERR_OK;
+    int sms = 0, dev = 0;
+    _CHECK(check_device(logits, &sms, &dev));
+    // the longest history that fits the small table with 512 biases
+    const uint32_t slots = !rules->history || rules->history_stride <= kSlotsSmall / 4 * 3 - 512 ? kSlotsSmall : kSlotsLarge;
+    RuleArgs a{*rules, logits, out, logits_stride, out_stride, vocab, rows, slots, 0, 0};
+    return dtype == vkllm_dtype_float16 ? launch_rules<__half>(a, sms, dev, (cudaStream_t)stream)
+                                        : launch_rules<float>(a, sms, dev, (cudaStream_t)stream);
 }

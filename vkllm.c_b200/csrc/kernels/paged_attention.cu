@@ -232,6 +232,7 @@ template <int HP, int NQ, bool EXACT> struct HalfCore
 {
     using T = __half;
     using S = Shape<T, HP>;
+    static constexpr int kQueries = 8 * NQ;
     static constexpr int kK = HP / 16;
     uint32_t qf[NQ][kK][2]; // Q^T as the B operand
     float o[NQ][kK][4], m[NQ][2], l[NQ][2];
@@ -368,29 +369,28 @@ template <int HP, int NQ, bool EXACT> struct HalfCore
 
 // fp32: 8 keys of a slice; lane = (part << 3) | key computes a quarter of that key's dot products (the
 // 16-byte pieces p with p % 4 == part); for the outputs a lane owns the pieces lane % kP, lane % kP + 32 ...
-template <int HP, bool EXACT> struct FloatCore
+template <int HP, int NQ, bool EXACT> struct FloatCore
 {
     using T = float;
     using S = Shape<T, HP>;
+    static constexpr int kQueries = NQ;
     static constexpr int kP = HP / 4;                       // pieces of a row
     static constexpr int kOwn = kP > 32 ? kP / 32 : 1;      // pieces that a lane owns
     static constexpr int kHalves = kP < 32 ? 32 / kP : 1;   // lane groups that share the keys (HP = 64: 2)
-    float4 o[8][kOwn];
-    float m[8], l[8];
-    uint32_t nq;
+    float4 o[NQ][kOwn];
+    float m[NQ], l[NQ];
 
-    __device__ __forceinline__ void start(const PagedAttArgs &a, uint32_t seq, uint32_t head0, uint32_t n, uint32_t lane,
+    __device__ __forceinline__ void start(const PagedAttArgs &a, uint32_t seq, uint32_t head0, uint32_t nq, uint32_t lane,
                                           float *qs)
     {
-        // the CTA's warps are at the same item here: each loads two of its queries
+        // the CTA's warps are at the same item here: each loads its share of the queries
         const uint32_t hd = a.kv.head_dim, warp = threadIdx.x >> 5;
-        nq = n;
-        for (uint32_t i = warp; i < 8; i += kWarps)
+        for (uint32_t i = warp; i < NQ; i += kWarps)
             for (uint32_t d = lane; d < HP; d += 32)
-                qs[i * HP + d] = i < n && d < hd ? ((const T *)a.q)[seq * a.q_stride + (uint64_t)(head0 + i) * hd + d] : 0.f;
+                qs[i * HP + d] = i < nq && d < hd ? ((const T *)a.q)[seq * a.q_stride + (uint64_t)(head0 + i) * hd + d] : 0.f;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < NQ; ++i)
         {
 #pragma unroll
             for (int k = 0; k < kOwn; ++k)
@@ -407,51 +407,62 @@ template <int HP, bool EXACT> struct FloatCore
         const float4 *K = reinterpret_cast<const float4 *>(sm + off);
         const float4 *V = K + S::kKeys * kP;
         const uint32_t key = lane & 7, part = lane >> 3;
-        float4 kr[kP / 4];
+        // every query's dot product in two chains (even and odd elements), all queries side by side
+        float d[NQ][2];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+            d[i][0] = d[i][1] = 0.f;
+        const uint32_t quads = EXACT ? kP / 4 : (a.kv.head_dim / 4 + 3) / 4; // quads of pieces that hold something
 #pragma unroll
         for (int j = 0; j < kP / 4; ++j)
-            kr[j] = K[key * kP + ((4 * j + part) ^ key)];
-        const bool in = (mask >> key) & 1u;
-        float p[8], f[8];
-        bool moved = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
         {
-            if (i >= nq)
+            if (!EXACT && j >= quads)
                 break;
-            float d = 0.f;
+            const float4 k = K[key * kP + ((4 * j + part) ^ key)];
 #pragma unroll
-            for (int j = 0; j < kP / 4; ++j)
+            for (int i = 0; i < NQ; ++i)
             {
                 const float4 q = reinterpret_cast<const float4 *>(qs + i * HP)[4 * j + part];
-                d = fmaf(q.x, kr[j].x, d), d = fmaf(q.y, kr[j].y, d);
-                d = fmaf(q.z, kr[j].z, d), d = fmaf(q.w, kr[j].w, d);
+                d[i][0] = fmaf(q.x, k.x, d[i][0]), d[i][1] = fmaf(q.y, k.y, d[i][1]);
+                d[i][0] = fmaf(q.z, k.z, d[i][0]), d[i][1] = fmaf(q.w, k.w, d[i][1]);
             }
-            d += __shfl_xor_sync(0xffffffffu, d, 8);
-            d += __shfl_xor_sync(0xffffffffu, d, 16);
-            const float x = in ? d * a.scale_log2 : -INFINITY;
-            float mx = x;
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, m[i]);
-            const float b = finite_base(mx);
+        }
+        const bool in = (mask >> key) & 1u;
+        float p[NQ], mx[NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+            p[i] = d[i][0] + d[i][1];
+#pragma unroll
+        for (int x = 8; x < 32; x <<= 1)
+#pragma unroll
+            for (int i = 0; i < NQ; ++i)
+                p[i] += __shfl_xor_sync(0xffffffffu, p[i], x);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+            mx[i] = p[i] = in ? p[i] * a.scale_log2 : -INFINITY;
+#pragma unroll
+        for (int x = 1; x < 8; x <<= 1)
+#pragma unroll
+            for (int i = 0; i < NQ; ++i)
+                mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], x));
+        bool moved = false;
+        float f[NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+        {
+            const float mn = fmaxf(mx[i], m[i]), b = finite_base(mn);
             f[i] = pow2(m[i] - b);
             moved |= f[i] != 1.f;
-            m[i] = mx;
-            p[i] = pow2(x - b);
+            m[i] = mn;
+            p[i] = pow2(p[i] - b);
             l[i] = fmaf(l[i], f[i], p[i]);
         }
         if (__any_sync(0xffffffffu, moved))
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-            {
-                if (i >= nq)
-                    break;
+            for (int i = 0; i < NQ; ++i)
 #pragma unroll
                 for (int k = 0; k < kOwn; ++k)
                     o[i][k].x *= f[i], o[i][k].y *= f[i], o[i][k].z *= f[i], o[i][k].w *= f[i];
-            }
         const uint32_t own = lane % kP, first = kHalves > 1 ? lane / kP : 0;
 #pragma unroll
         for (uint32_t j = 0; j < S::kKeys / kHalves; ++j)
@@ -462,10 +473,8 @@ template <int HP, bool EXACT> struct FloatCore
             for (int k = 0; k < kOwn; ++k)
                 v[k] = V[r * kP + ((own + 32 * k) ^ (r & 7))];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < NQ; ++i)
             {
-                if (i >= nq)
-                    break;
                 const float w = __shfl_sync(0xffffffffu, p[i], r);
 #pragma unroll
                 for (int k = 0; k < kOwn; ++k)
@@ -480,7 +489,7 @@ template <int HP, bool EXACT> struct FloatCore
     __device__ __forceinline__ void deposit(int, float *os, float *ml, uint32_t lane)
     {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < NQ; ++i)
         {
             float t = l[i];
             t += __shfl_xor_sync(0xffffffffu, t, 1);
@@ -547,11 +556,13 @@ __device__ __forceinline__ void join_warps(const PagedAttArgs &a, const float *o
     }
 }
 
-template <typename Core, typename T, int HP, int NQ, bool EXACT>
+template <template <int, int, bool> class Kind, typename T, int HP, int NQ, bool EXACT>
 __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attention(const PagedAttArgs a)
 {
     using S = Shape<T, HP>;
+    using Core = Kind<HP, NQ, EXACT>;
     constexpr uint32_t kTile = kWarps * S::kKeys;
+    constexpr int kRounds = (Core::kQueries + 7) / 8; // the join buffer takes 8 queries at a time
     extern __shared__ __align__(128) unsigned char sm[];
     float *qs = reinterpret_cast<float *>(sm + S::kRing);
     float *os = reinterpret_cast<float *>(sm + S::kRing + S::kQBytes); // [kWarps][8][kPitch]
@@ -674,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
         // a part goes to the CTA's first slot when the item began before, else to its second
         float *part = whole ? nullptr : a.parts + (2 * (uint64_t)blockIdx.x + (from == 0)) * a.part_stride;
 #pragma unroll
-        for (int r = 0; r < NQ; ++r)
+        for (int r = 0; r < kRounds; ++r)
         {
             if (r * 8 >= nq)
                 break;
@@ -753,11 +764,11 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
         atomicOr(a.status, ld.status);
 }
 
-template <typename Core, typename T, int HP, int NQ, bool EXACT>
+template <template <int, int, bool> class Kind, typename T, int HP, int NQ, bool EXACT>
 vkllm_err_t launch(PagedAttArgs &a, int sms, int device, cudaStream_t s)
 {
     using S = Shape<T, HP>;
-    auto kernel = k_paged_attention<Core, T, HP, NQ, EXACT>;
+    auto kernel = k_paged_attention<Kind, T, HP, NQ, EXACT>;
     static std::atomic<bool> done[64]; // the attribute of this kernel, set once a device (twice does no harm)
     if (device >= 64 || !done[device].load(std::memory_order_relaxed))
     {
@@ -780,17 +791,21 @@ vkllm_err_t launch(PagedAttArgs &a, int sms, int device, cudaStream_t s)
     return VKLLM_ERR_OK;
 }
 
+template <template <int, int, bool> class Kind, typename T, int HP, int NQ>
+vkllm_err_t launch_exact(PagedAttArgs &a, int sms, int device, cudaStream_t s)
+{
+    return a.kv.head_dim == HP ? launch<Kind, T, HP, NQ, true>(a, sms, device, s)
+                               : launch<Kind, T, HP, NQ, false>(a, sms, device, s);
+}
+
 template <int HP> vkllm_err_t launch_head(PagedAttArgs &a, int sms, int device, cudaStream_t s)
 {
-    const bool exact = a.kv.head_dim == HP;
-    if (a.kv.dtype == vkllm_dtype_float32)
-        return exact ? launch<FloatCore<HP, true>, float, HP, 1, true>(a, sms, device, s)
-                     : launch<FloatCore<HP, false>, float, HP, 1, false>(a, sms, device, s);
-    if (a.gq <= 8)
-        return exact ? launch<HalfCore<HP, 1, true>, __half, HP, 1, true>(a, sms, device, s)
-                     : launch<HalfCore<HP, 1, false>, __half, HP, 1, false>(a, sms, device, s);
-    return exact ? launch<HalfCore<HP, 2, true>, __half, HP, 2, true>(a, sms, device, s)
-                 : launch<HalfCore<HP, 2, false>, __half, HP, 2, false>(a, sms, device, s);
+    if (a.kv.dtype == vkllm_dtype_float16)
+        return a.gq <= 8 ? launch_exact<HalfCore, __half, HP, 1>(a, sms, device, s)
+                         : launch_exact<HalfCore, __half, HP, 2>(a, sms, device, s);
+    return a.gq == 1   ? launch_exact<FloatCore, float, HP, 1>(a, sms, device, s)
+           : a.gq <= 4 ? launch_exact<FloatCore, float, HP, 4>(a, sms, device, s)
+                       : launch_exact<FloatCore, float, HP, 8>(a, sms, device, s);
 }
 
 } // namespace
