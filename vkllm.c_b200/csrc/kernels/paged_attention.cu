@@ -8,11 +8,12 @@
 //
 // Work. Lengths are known on the device only, so the kernel divides the work itself. An item is one
 // (sequence, key head, tile of up to 8 or 16 of its queries); its keys are cut into tiles of 4 slices,
-// one slice per warp (16 keys in fp16, 8 in fp32). All tiles of all items form one line, of which every CTA
-// of a grid that fills the GPU takes an equal part: a long sequence spreads over all SMs and short ones
-// share a CTA. A CTA that holds only a part of an item leaves (m, l, O) in the workspace and counts
+// one slice per warp (16 keys in fp16, 8 in fp32). All tiles of all items form one line, in which an item's end
+// counts too, and every CTA of a grid that fills the GPU takes an equal part of it: a long sequence spreads over all SMs and
+// short ones share a CTA. A CTA that holds only a part of an item leaves (m, l, O) in the workspace and counts
 // itself at the item; the last one to arrive joins the parts in the order of the line, so the result
-// does not depend on who was last.
+// does not depend on who was last. (Handing the last quarter of the line out in small chunks off a ticket
+// counter was slower: 98 instead of 78 us for 64 sequences of 128 to 640 keys, since every chunk refills the rings.)
 //
 // Loads. Each warp streams its own slices through a private ring of cp.async stages, also across the
 // borders of items: no barrier of the CTA stands between a load and its use. Page ids are read one tile ahead of
@@ -37,7 +38,9 @@ namespace
 
 constexpr uint32_t kWarps = 4, kThreads = kWarps * 32;
 constexpr uint32_t kCounters = 1024;      // words at the start of the workspace, one per CTA of the grid
-constexpr uint32_t kMinTiles = 4;         // least tiles of a CTA (see launch)
+// Lengths on the line: a tile, and what an item costs beside its tiles (its queries read, its warps joined).
+constexpr uint32_t kTileUnits = 4, kItemUnits = 6;
+constexpr uint32_t kMinUnits = 2 * kTileUnits + kItemUnits; // least part of a CTA: an item of two tiles
 constexpr float kWeightShift = 15.f;      // weights are at most 2^15, below fp16's 65504
 
 struct PagedAttArgs
@@ -61,16 +64,19 @@ struct PagedAttArgs
     uint32_t part_stride;
 };
 
+constexpr uint32_t kRound = 4; // queries that the join buffers take at a time
+
 template <typename T, int HP> struct Shape
 {
     static constexpr uint32_t kKeys = sizeof(T) == 2 ? 16 : 8;                  // keys of a slice
     static constexpr uint32_t kRow = HP * sizeof(T);                            // bytes of a row in shared memory
     static constexpr uint32_t kStage = 2 * kKeys * kRow;                        // K and V of a slice
     static constexpr uint32_t kQBytes = sizeof(T) == 4 ? 8 * HP * 4 : 0;        // the queries (fp32 only)
-    static constexpr uint32_t kStages = HP == 64 ? 6 : (HP == 256 && sizeof(T) == 4) ? 2 : 3;
+    static constexpr uint32_t kStages = sizeof(T) == 4 ? (HP == 64 ? 4 : 2) : HP == 64 ? 6 : 3;
     static constexpr uint32_t kPitch = HP + 4;                                  // floats of a row of the join buffer
     static constexpr uint32_t kRing = kWarps * kStages * kStage;
-    static constexpr uint32_t kSmem = kRing + kQBytes + kWarps * 8 * kPitch * 4 + kWarps * 8 * 2 * 4 + kWarps * kStages * 4;
+    static constexpr uint32_t kJoin = kWarps * kRound * (kPitch + 2);           // floats of a join buffer: O, then m and l
+    static constexpr uint32_t kSmem = kRing + kQBytes + 2 * kJoin * 4 + kWarps * kStages * 4;
     static constexpr uint32_t kCtas = HP == 256 ? 1 : 2; // per SM
 };
 
@@ -133,21 +139,33 @@ __device__ __forceinline__ float finite_base(float m)
     return m == -INFINITY ? 0.f : m;
 }
 
-// A place in the line of tiles: tile `tile` of `tiles` of item (seq, hq), hq = key head * qtiles + query tile.
+__host__ __device__ __forceinline__ uint32_t item_units(uint32_t tiles)
+{
+    return tiles ? tiles * kTileUnits + kItemUnits : 0;
+}
+
+// A place in the line of tiles: tile `tile` of `tiles` of item (seq, hq), hq = key head * qtiles + query tile, `unit`
+// units behind the start of the CTA's part.
 struct Cursor
 {
-    uint32_t seq, hq, tile, tiles, len;
+    uint32_t seq, hq, tile, tiles, len, unit;
 
     __device__ __forceinline__ void set_len(const PagedAttArgs &a, uint32_t tile_keys)
     {
         len = min(a.lens[seq], a.cap);
         tiles = (len + tile_keys - 1) / tile_keys;
     }
-    // One tile on; stays at the last item's end when there is no further one.
+    // One tile on; behind the last one seq is n_seqs.
     __device__ __forceinline__ void next(const PagedAttArgs &a, uint32_t items, uint32_t tile_keys)
     {
-        if (++tile < tiles)
-            return;
+        unit += kTileUnits;
+        if (++tile >= tiles)
+            next_item(a, items, tile_keys);
+    }
+    // From behind the last tile to the first of the next item.
+    __device__ __forceinline__ void next_item(const PagedAttArgs &a, uint32_t items, uint32_t tile_keys)
+    {
+        unit += kItemUnits;
         tile = 0;
         if (++hq < items)
             return;
@@ -164,7 +182,7 @@ template <typename T, int HP, bool EXACT> struct Loader
     using S = Shape<T, HP>;
     static constexpr uint32_t kPieces = S::kRow / 16;
     Cursor c;
-    uint32_t left; // tiles still to load
+    uint32_t end;  // units of the CTA's part
     uint32_t page; // of key `lane % kKeys` of the slice at c
     uint32_t ring; // shared address of the warp's ring
     uint32_t *valid; // [kStages] masks of the slice's keys that count
@@ -174,15 +192,27 @@ template <typename T, int HP, bool EXACT> struct Loader
     {
         return (c.tile * kWarps + warp) * S::kKeys + lane % S::kKeys;
     }
+    __device__ __forceinline__ bool more(const PagedAttArgs &a) const
+    {
+        return c.unit < end && c.seq < a.n_seqs;
+    }
     __device__ __forceinline__ void lookup(const PagedAttArgs &a, uint32_t warp, uint32_t lane)
     {
         const uint32_t k = key(warp, lane);
-        page = left && k < c.len ? __ldg(a.table + c.seq * a.table_stride + k / a.kv.page_rows) : 0xffffffffu;
+        page = more(a) && k < c.len ? __ldg(a.table + c.seq * a.table_stride + k / a.kv.page_rows) : 0xffffffffu;
+    }
+    __device__ __forceinline__ void prefetch_queries(const PagedAttArgs &a, uint32_t lane) const
+    {
+        const uint32_t qt = c.hq % a.qtiles, nq = min(a.gq, a.group - qt * a.gq);
+        const char *q = (const char *)((const T *)a.q + c.seq * a.q_stride +
+                                       (uint64_t)(c.hq / a.qtiles * a.group + qt * a.gq) * a.kv.head_dim);
+        for (uint32_t b = lane * 128; b < nq * a.kv.head_dim * (uint32_t)sizeof(T); b += 32 * 128)
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(q + b));
     }
     // Issues the slice at c as one group of copies (an empty one behind the end) and moves on.
     __device__ __forceinline__ void issue(const PagedAttArgs &a, uint32_t items, uint32_t warp, uint32_t lane)
     {
-        if (left)
+        if (more(a))
         {
             const uint32_t k = key(warp, lane);
             bool ok = k < c.len;
@@ -204,6 +234,8 @@ template <typename T, int HP, bool EXACT> struct Loader
 #pragma unroll
                 for (uint32_t i = 0; i < kMost; ++i)
                 {
+                    if (!EXACT && i * 32 >= S::kKeys * pieces)
+                        break;
                     const uint32_t r = row % S::kKeys; // row < kKeys for every copy that is made
                     const uint64_t off = __shfl_sync(0xffffffffu, at, r) + p * (16 / sizeof(T));
                     const uint32_t bytes = (mask >> r) & 1u ? 16u : 0u;
@@ -218,9 +250,10 @@ template <typename T, int HP, bool EXACT> struct Loader
                         p -= pieces, ++row;
                 }
             }
-            --left;
             c.next(a, items, kWarps * S::kKeys);
             lookup(a, warp, lane);
+            if (c.tile == 0 && more(a)) // a new item ahead: its queries will be wanted
+                prefetch_queries(a, lane);
         }
         cp_commit();
         stage = stage + 1 == S::kStages ? 0 : stage + 1;
@@ -339,28 +372,31 @@ template <int HP, int NQ, bool EXACT> struct HalfCore
         }
     }
 
-    // Queries 8 n .. 8 n + 7 into the join buffer: os [8][kPitch], ml [8][2].
-    __device__ __forceinline__ void deposit(int n, float *os, float *ml, uint32_t lane)
+    // Queries kRound r .. of the item, those below nq, into the warp's join buffer: os [kRound][kPitch], ml [kRound][2].
+    __device__ __forceinline__ void deposit(int r, uint32_t nq, float *os, float *ml, uint32_t lane)
     {
 #pragma unroll
-        for (int nn = 0; nn < NQ; ++nn)
-            if (nn == n)
+        for (int n = 0; n < NQ; ++n)
+            if (n == r / 2)
             {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                 {
-                    const uint32_t q = (lane & 3) * 2 + i;
-                    float t = l[nn][i];
+                    float t = l[n][i];
                     t += __shfl_xor_sync(0xffffffffu, t, 4);
                     t += __shfl_xor_sync(0xffffffffu, t, 8);
                     t += __shfl_xor_sync(0xffffffffu, t, 16);
+                    // this lane's query is 8 n + 2 (lane & 3) + i
+                    const uint32_t q = (lane & 1) * 2 + i;
+                    if ((lane >> 1 & 1u) != (uint32_t)(r & 1) || r * kRound + q >= nq)
+                        continue;
                     if (lane < 4)
-                        ml[q * 2] = m[nn][i], ml[q * 2 + 1] = t;
+                        ml[q * 2] = m[n][i], ml[q * 2 + 1] = t;
 #pragma unroll
                     for (int k = 0; k < kK; ++k)
                     {
-                        os[q * S::kPitch + k * 16 + (lane >> 2)] = o[nn][k][i];
-                        os[q * S::kPitch + k * 16 + (lane >> 2) + 8] = o[nn][k][i + 2];
+                        os[q * S::kPitch + k * 16 + (lane >> 2)] = o[n][k][i];
+                        os[q * S::kPitch + k * 16 + (lane >> 2) + 8] = o[n][k][i + 2];
                     }
                 }
             }
@@ -486,17 +522,20 @@ template <int HP, int NQ, bool EXACT> struct FloatCore
         }
     }
 
-    __device__ __forceinline__ void deposit(int, float *os, float *ml, uint32_t lane)
+    __device__ __forceinline__ void deposit(int r, uint32_t nq, float *os, float *ml, uint32_t lane)
     {
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
         {
+            if (i / kRound != r || i >= nq)
+                continue;
+            const uint32_t q = i % kRound;
             float t = l[i];
             t += __shfl_xor_sync(0xffffffffu, t, 1);
             t += __shfl_xor_sync(0xffffffffu, t, 2);
             t += __shfl_xor_sync(0xffffffffu, t, 4);
             if (lane == 0)
-                ml[i * 2] = m[i], ml[i * 2 + 1] = t;
+                ml[q * 2] = m[i], ml[q * 2 + 1] = t;
 #pragma unroll
             for (int k = 0; k < kOwn; ++k)
             {
@@ -507,71 +546,161 @@ template <int HP, int NQ, bool EXACT> struct FloatCore
                     v.z += __shfl_xor_sync(0xffffffffu, v.z, 16), v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
                 }
                 if (kHalves == 1 || lane < kP)
-                    *reinterpret_cast<float4 *>(os + i * S::kPitch + 4 * (lane % kP + 32 * k)) = v;
+                    *reinterpret_cast<float4 *>(os + q * S::kPitch + 4 * (lane % kP + 32 * k)) = v;
             }
         }
     }
 };
 
-// The queries of the join buffer, joined over its warps: `gq` queries from query q0 of the item, to the output or to a part.
+template <typename T>
+__device__ __forceinline__ void store_out(const PagedAttArgs &a, uint32_t seq, uint32_t head, uint32_t d, float4 o, float l)
+{
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T *dst = (T *)a.out + seq * a.out_stride + (uint64_t)head * a.kv.head_dim + d;
+    if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
+    else
+        *reinterpret_cast<float4 *>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+__device__ __forceinline__ void add_scaled(float4 &o, float f, const float4 &v)
+{
+    o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+}
+
+// A join buffer, joined over the warps: queries q0 .. q0 + n - 1 of the item (at most kRound), to the output or to a part.
 template <typename T, int HP>
-__device__ __forceinline__ void join_warps(const PagedAttArgs &a, const float *os, const float *ml, uint32_t gq,
-                                           uint32_t q0, uint32_t seq, uint32_t head0, float *part, uint32_t part_q)
+__device__ __forceinline__ void join_warps(const PagedAttArgs &a, const float *os, const float *ml, uint32_t n,
+                                           uint32_t q0, uint32_t seq, uint32_t head0, float *part)
 {
     using S = Shape<T, HP>;
-    const uint32_t hd = a.kv.head_dim;
-    for (uint32_t i = threadIdx.x; i < gq * (HP / 4); i += kThreads)
+    for (uint32_t i = threadIdx.x; i < n * (HP / 4); i += kThreads)
     {
         const uint32_t q = i / (HP / 4), d = i % (HP / 4) * 4;
         float mx = -INFINITY;
 #pragma unroll
         for (uint32_t w = 0; w < kWarps; ++w)
-            mx = fmaxf(mx, ml[(w * 8 + q) * 2]);
+            mx = fmaxf(mx, ml[(w * kRound + q) * 2]);
         const float b = finite_base(mx);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         float l = 0.f;
 #pragma unroll
         for (uint32_t w = 0; w < kWarps; ++w)
         {
-            const float f = pow2(ml[(w * 8 + q) * 2] - b);
-            const float4 v = *reinterpret_cast<const float4 *>(os + (w * 8 + q) * S::kPitch + d);
-            l = fmaf(f, ml[(w * 8 + q) * 2 + 1], l);
-            o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+            const float f = pow2(ml[(w * kRound + q) * 2] - b);
+            l = fmaf(f, ml[(w * kRound + q) * 2 + 1], l);
+            add_scaled(o, f, *reinterpret_cast<const float4 *>(os + (w * kRound + q) * S::kPitch + d));
         }
         if (part)
         {
             *reinterpret_cast<float4 *>(part + (q0 + q) * HP + d) = o;
             if (d == 0)
-                part[part_q * HP + q0 + q] = mx, part[part_q * (HP + 1) + q0 + q] = l;
+                part[a.gq * HP + q0 + q] = mx, part[a.gq * (HP + 1) + q0 + q] = l;
         }
-        else if (d < hd)
-        {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            T *dst = (T *)a.out + seq * a.out_stride + (uint64_t)(head0 + q0 + q) * hd + d;
-            if constexpr (sizeof(T) == 2)
-                *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
-            else
-                *reinterpret_cast<float4 *>(dst) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        }
+        else if (d < a.kv.head_dim)
+            store_out<T>(a, seq, head0 + q0 + q, d, o, l);
     }
 }
 
+// The part of CTA c of an item that begins in CTA c0: a CTA's second place is for the item that begins in it and goes on.
+__device__ __forceinline__ float *part_of(const PagedAttArgs &a, uint32_t c, bool begins)
+{
+    return a.parts + (2 * (uint64_t)c + begins) * a.part_stride;
+}
+
+// An item joined over its parts in CTAs c0 .. c1, in their order, to the output. What it costs is the latency of its loads, at
+// the end of a CTA's work: so every thread takes 4 elements of a query with the statistics of their parts on its
+// own, 16 parts in flight, and where the item has too few elements to fill the CTA, and parts enough, groups of
+// threads take every `groups`-th part and meet in shared memory.
+template <typename T, int HP>
+__device__ __noinline__ void join_parts(const PagedAttArgs &a, uint32_t c0, uint32_t c1, float *sm, uint32_t nq,
+                                        uint32_t seq, uint32_t head0)
+{
+    constexpr uint32_t kCols = HP / 4, kAhead = 16;
+    const uint32_t cols = nq * kCols, np = c1 - c0 + 1;
+    const uint32_t groups = np > kAhead && cols < kThreads ? kThreads / cols : 1;
+    const uint32_t group = groups > 1 ? threadIdx.x / cols : 0;
+    for (uint32_t c = threadIdx.x - group * cols; c < cols && group < groups; c += groups > 1 ? cols : kThreads)
+    {
+        const uint32_t q = c / kCols, d = c % kCols * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float mx = -INFINITY, l = 0.f;
+        for (uint32_t p0 = c0 + group; p0 <= c1; p0 += groups * kAhead)
+        {
+            float m[kAhead], pl[kAhead], top = mx;
+            float4 v[kAhead];
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u)
+            {
+                const uint32_t p = p0 + u * groups;
+                m[u] = -INFINITY, pl[u] = 0.f, v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (p > c1)
+                    continue;
+                const float *src = part_of(a, p, p == c0);
+                m[u] = __ldcg(src + a.gq * HP + q), pl[u] = __ldcg(src + a.gq * (HP + 1) + q);
+                v[u] = __ldcg(reinterpret_cast<const float4 *>(src + q * HP + d));
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u)
+                top = fmaxf(top, m[u]);
+            const float b = finite_base(top), f = pow2(mx - b);
+            mx = top;
+            l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u)
+            {
+                const float g = pow2(m[u] - b);
+                l = fmaf(g, pl[u], l);
+                add_scaled(o, g, v[u]);
+            }
+        }
+        if (groups > 1)
+        {
+            float *row = sm + (group * cols + c) * 8;
+            *reinterpret_cast<float4 *>(row) = o;
+            row[4] = mx, row[5] = l;
+        }
+        else if (d < a.kv.head_dim)
+            store_out<T>(a, seq, head0 + q, d, o, l);
+    }
+    if (groups == 1)
+        return;
+    __syncthreads();
+    if (threadIdx.x < cols)
+    {
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float mx = -INFINITY, l = 0.f;
+        for (uint32_t g = 0; g < groups; ++g)
+            mx = fmaxf(mx, sm[(g * cols + threadIdx.x) * 8 + 4]);
+        const float b = finite_base(mx);
+        for (uint32_t g = 0; g < groups; ++g)
+        {
+            const float *row = sm + (g * cols + threadIdx.x) * 8;
+            const float f = pow2(row[4] - b);
+            l = fmaf(f, row[5], l);
+            add_scaled(o, f, *reinterpret_cast<const float4 *>(row));
+        }
+        if (threadIdx.x % kCols * 4 < a.kv.head_dim)
+            store_out<T>(a, seq, head0 + threadIdx.x / kCols, threadIdx.x % kCols * 4, o, l);
+    }
+    __syncthreads();
+}
+
 template <template <int, int, bool> class Kind, typename T, int HP, int NQ, bool EXACT>
-__global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attention(const PagedAttArgs a)
+__global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attention(const __grid_constant__ PagedAttArgs a)
 {
     using S = Shape<T, HP>;
     using Core = Kind<HP, NQ, EXACT>;
     constexpr uint32_t kTile = kWarps * S::kKeys;
-    constexpr int kRounds = (Core::kQueries + 7) / 8; // the join buffer takes 8 queries at a time
+    constexpr int kRounds = (Core::kQueries + kRound - 1) / kRound;
     extern __shared__ __align__(128) unsigned char sm[];
     float *qs = reinterpret_cast<float *>(sm + S::kRing);
-    float *os = reinterpret_cast<float *>(sm + S::kRing + S::kQBytes); // [kWarps][8][kPitch]
-    float *ml = os + kWarps * 8 * S::kPitch;                           // [kWarps][8][2]
-    uint32_t *valid = reinterpret_cast<uint32_t *>(ml + kWarps * 8 * 2); // [kWarps][kStages]
+    float *join = reinterpret_cast<float *>(sm + S::kRing + S::kQBytes); // two buffers: one is joined while the other fills
+    uint32_t *valid = reinterpret_cast<uint32_t *>(join + 2 * S::kJoin); // [kWarps][kStages]
     __shared__ uint64_t sums[kWarps];
     __shared__ Cursor first;
     __shared__ uint32_t last_one;
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = a.kv.head_dim;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t items = a.kv.kv_heads * a.qtiles; // of a sequence
     if (!EXACT) // the pieces behind head_dim are never loaded: they have to be zeros, not whatever was there
         for (uint32_t i = tid; i < S::kRing / 16; i += kThreads)
@@ -590,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
         {
             if (len > a.cap)
                 status = VKLLM_B200_PAGED_TOO_LONG;
-            mine += (min(len, a.cap) + kTile - 1) / kTile;
+            mine += item_units((min(len, a.cap) + kTile - 1) / kTile);
         }
         uint32_t empty = __ballot_sync(0xffffffffu, len == 0 && s % gridDim.x == blockIdx.x);
         while (empty)
@@ -598,10 +727,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
             const uint32_t z = __shfl_sync(0xffffffffu, s, __ffs(empty) - 1);
             empty &= empty - 1;
             uint4 *row = reinterpret_cast<uint4 *>((T *)a.out + z * a.out_stride);
-            for (uint32_t d = lane; d < a.kv.kv_heads * a.group * hd * sizeof(T) / 16; d += 32)
+            for (uint32_t d = lane; d < a.kv.kv_heads * a.group * a.kv.head_dim * (uint32_t)sizeof(T) / 16; d += 32)
                 row[d] = make_uint4(0, 0, 0, 0);
         }
     }
+    if (status)
+        atomicOr(a.status, status);
+    mine *= items;
     uint64_t before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1)
@@ -622,30 +754,35 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
             before += sums[w];
         total += sums[w];
     }
-    total *= items;
-    before *= items;
-    mine *= items;
-    const uint64_t share = (total + gridDim.x - 1) / gridDim.x, per = share < kMinTiles ? kMinTiles : share;
-    const uint64_t begin = blockIdx.x * per, end = begin + per < total ? begin + per : total;
-    if (status)
-        atomicOr(a.status, status);
+    const uint64_t per = max((total + gridDim.x - 1) / gridDim.x, (uint64_t)kMinUnits);
+    const uint64_t begin = blockIdx.x * per;
     if (begin >= total)
         return;
+    const uint32_t end = (uint32_t)min(per, total - begin);
     if (before <= begin && begin < before + mine)
     {
         Cursor c;
         c.seq = tid * per_thread;
         uint64_t at = before;
+        uint32_t units = 0;
         for (; c.seq < a.n_seqs; ++c.seq)
         {
             c.set_len(a, kTile);
-            const uint64_t n = (uint64_t)c.tiles * items;
-            if (begin < at + n)
+            units = item_units(c.tiles);
+            if (begin < at + (uint64_t)units * items)
                 break;
-            at += n;
+            at += (uint64_t)units * items;
         }
-        c.hq = (uint32_t)((begin - at) / c.tiles);
-        c.tile = (uint32_t)((begin - at) % c.tiles);
+        units = max(units, 1u);
+        c.hq = (uint32_t)((begin - at) / units);
+        const uint32_t x = (uint32_t)((begin - at) % units); // a tile is the CTA's in whose part its first unit lies
+        c.tile = (x + kTileUnits - 1) / kTileUnits;
+        c.unit = c.tile * kTileUnits - x;
+        if (c.tile >= c.tiles)
+        {
+            c.unit = units - x - kItemUnits; // modulo 2^32: next_item adds them again
+            c.next_item(a, items, kTile);
+        }
         first = c;
     }
     __syncthreads();
@@ -653,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
     Cursor c = first;
     Loader<T, HP, EXACT> ld;
     ld.c = c;
-    ld.left = (uint32_t)(end - begin);
+    ld.end = end;
     ld.ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * S::kStages * S::kStage;
     ld.valid = valid + warp * S::kStages;
     ld.lookup(a, warp, lane);
@@ -662,12 +799,11 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
         ld.issue(a, items, warp, lane);
 
     Core core;
-    uint32_t stage = 0;
-    uint64_t at = begin;
-    while (at < end && c.seq < a.n_seqs) // (the second holds unless lens is written meanwhile)
+    uint32_t stage = 0, buffer = 0;
+    while (c.unit < end && c.seq < a.n_seqs)
     {
         // one item, or this CTA's part of it
-        const uint32_t tiles = c.tiles, from = c.tile, n = (uint32_t)min((uint64_t)(tiles - from), end - at);
+        const uint32_t from = c.tile, n = min(c.tiles - from, (end - c.unit + kTileUnits - 1) / kTileUnits);
         const uint32_t qt = c.hq % a.qtiles, head0 = c.hq / a.qtiles * a.group + qt * a.gq;
         const uint32_t nq = min(a.gq, a.group - qt * a.gq);
         core.start(a, c.seq, head0, nq, lane, qs);
@@ -681,84 +817,43 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
                 core.slice(a, ld.ring + stage * S::kStage, mask, lane, qs);
             stage = stage + 1 == S::kStages ? 0 : stage + 1;
         }
-        const bool whole = n == tiles;
-        // a part goes to the CTA's first slot when the item began before, else to its second
-        float *part = whole ? nullptr : a.parts + (2 * (uint64_t)blockIdx.x + (from == 0)) * a.part_stride;
+        const bool whole = n == c.tiles;
+        float *part = whole ? nullptr : part_of(a, blockIdx.x, from == 0);
 #pragma unroll
         for (int r = 0; r < kRounds; ++r)
         {
-            if (r * 8 >= nq)
+            if (r * kRound >= nq)
                 break;
-            core.deposit(r, os + warp * 8 * S::kPitch, ml + warp * 8 * 2, lane);
+            // the barrier also says that every warp is done with the other buffer
+            float *os = join + buffer * S::kJoin, *ml = os + kWarps * kRound * S::kPitch;
+            core.deposit(r, nq, os + warp * kRound * S::kPitch, ml + warp * kRound * 2, lane);
             __syncthreads();
-            join_warps<T, HP>(a, os, ml, min(nq - r * 8, 8u), r * 8, c.seq, head0, part, a.gq);
-            __syncthreads();
+            join_warps<T, HP>(a, os, ml, min(nq - r * kRound, kRound), r * kRound, c.seq, head0, part);
+            buffer ^= 1;
         }
         if (!whole)
         {
             // CTAs c0 .. c1 hold the item's parts
-            const uint64_t item = at - from;
-            const uint32_t c0 = (uint32_t)(item / per), c1 = (uint32_t)((item + tiles - 1) / per);
-            __threadfence();
+            const uint64_t item = begin + c.unit - from * kTileUnits;
+            const uint32_t c0 = (uint32_t)(item / per), c1 = (uint32_t)((item + (c.tiles - 1) * (uint64_t)kTileUnits) / per);
             __syncthreads();
             if (tid == 0)
+            {
+                __threadfence(); // the part, which the barrier made this thread's to publish, before the count
                 last_one = atomicAdd(a.counters + c0, 1u) == c1 - c0;
+                __threadfence();
+            }
             __syncthreads();
             if (last_one)
             {
-                __threadfence();
                 if (tid == 0)
                     a.counters[c0] = 0; // ready for the next call
-                for (uint32_t r = 0; r * 8 < nq; ++r)
-                {
-                    // each warp joins every fourth part of 8 queries, then the warps join as above
-                    const uint32_t gq = min(nq - r * 8, 8u);
-                    for (uint32_t q = 0; q < gq; ++q)
-                    {
-                        constexpr int kOwn = HP > 128 ? HP / 128 : 1;
-                        float mx = -INFINITY, l = 0.f;
-                        float4 o[kOwn];
-#pragma unroll
-                        for (int k = 0; k < kOwn; ++k)
-                            o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        const bool lane_on = HP >= 128 || lane < HP / 4;
-#pragma unroll 4
-                        for (uint32_t p = c0 + warp; p <= c1; p += kWarps)
-                        {
-                            const float *src = a.parts + (2 * (uint64_t)p + (p == c0)) * a.part_stride;
-                            const float pm = __ldcg(src + a.gq * HP + r * 8 + q), pl = __ldcg(src + a.gq * (HP + 1) + r * 8 + q);
-                            float4 v[kOwn];
-#pragma unroll
-                            for (int k = 0; k < kOwn; ++k)
-                                v[k] = lane_on ? __ldcg(reinterpret_cast<const float4 *>(src + (r * 8 + q) * HP) + lane + 32 * k)
-                                               : make_float4(0.f, 0.f, 0.f, 0.f);
-                            const float mn = fmaxf(mx, pm), b = finite_base(mn), f = pow2(mx - b), g = pow2(pm - b);
-                            mx = mn;
-                            l = l * f + pl * g;
-#pragma unroll
-                            for (int k = 0; k < kOwn; ++k)
-                            {
-                                o[k].x = o[k].x * f + v[k].x * g, o[k].y = o[k].y * f + v[k].y * g;
-                                o[k].z = o[k].z * f + v[k].z * g, o[k].w = o[k].w * f + v[k].w * g;
-                            }
-                        }
-                        if (lane_on)
-#pragma unroll
-                            for (int k = 0; k < kOwn; ++k)
-                                *reinterpret_cast<float4 *>(os + (warp * 8 + q) * S::kPitch + 4 * (lane + 32 * k)) = o[k];
-                        if (lane == 0)
-                            ml[(warp * 8 + q) * 2] = mx, ml[(warp * 8 + q) * 2 + 1] = l;
-                    }
-                    __syncthreads();
-                    join_warps<T, HP>(a, os, ml, gq, r * 8, c.seq, head0, nullptr, 0);
-                    __syncthreads();
-                }
+                join_parts<T, HP>(a, c0, c1, join, nq, c.seq, head0);
             }
         }
-        at += n;
         c.tile = from + n - 1;
-        if (at < end)
-            c.next(a, items, kTile);
+        c.unit += (n - 1) * kTileUnits;
+        c.next(a, items, kTile);
     }
     if (ld.status)
         atomicOr(a.status, ld.status);
@@ -779,8 +874,9 @@ vkllm_err_t launch(PagedAttArgs &a, int sms, int device, cudaStream_t s)
     a.part_stride = a.gq * (HP + 2);
     a.part_stride = (a.part_stride + 3) / 4 * 4;
     // most CTAs that can have work, that the counters and the workspace serve, and that the GPU holds at once
-    const uint64_t tiles = (a.cap + (uint64_t)kWarps * S::kKeys - 1) / (kWarps * S::kKeys);
-    const uint64_t work = (tiles * a.n_seqs * a.kv.kv_heads * a.qtiles + kMinTiles - 1) / kMinTiles;
+    const uint32_t tiles = (uint32_t)((a.cap + (uint64_t)kWarps * S::kKeys - 1) / (kWarps * S::kKeys));
+    const uint64_t units = (uint64_t)tiles * kTileUnits + kItemUnits;
+    const uint64_t work = (units * a.n_seqs * a.kv.kv_heads * a.qtiles + kMinUnits - 1) / kMinUnits;
     const uint64_t room = (VKLLM_B200_PAGED_WORKSPACE_BYTES - kCounters * 4) / (2 * (uint64_t)a.part_stride * 4);
     uint64_t grid = (uint64_t)sms * S::kCtas;
     grid = grid < work ? grid : work;
