@@ -12,8 +12,9 @@
 // rounded f: an error of at most position * 2^-64 turns, and no range reduction. sincospif takes it
 // from there in fp32.
 //
-// Each thread owns one 16-byte piece of a head (4 or 2 pairs), so its sines and cosines serve every head
-// that it walks over.
+// A block works out a token's sines and cosines once, into shared memory; each thread owns one 16-byte piece of a
+// head (4 or 2 pairs), keeps those of its pairs, and walks over its share of the token's heads, 4 loads in flight.
+// 2048 tokens of 40 + 80 heads of 128 (126 MB, fp16): 24.6 us, 5.1 TB/s, where a plain copy of 102 MB reaches 5.5.
 #include <cmath>
 
 #include "paged.cuh"
@@ -25,6 +26,7 @@ namespace
 {
 
 constexpr uint32_t kRopeThreads = 256;
+constexpr uint32_t kRopeAhead = 4; // rows of a thread in flight
 
 struct RopeArgs
 {
@@ -79,6 +81,7 @@ template <> struct Piece<float>
 template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_rope_write(const RopeArgs a)
 {
     constexpr int P = Piece<T>::kPairs, E = 2 * P;
+    __shared__ __align__(16) float2 table[128]; // (cos, sin) of every pair of a head at the token's position
     const uint32_t t = blockIdx.x, slot = a.slots[t];
     if (slot == VKLLM_B200_NO_SLOT)
         return;
@@ -91,46 +94,56 @@ template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_ro
     }
     const uint32_t hd = a.kv.head_dim, pieces = hd / E, piece = threadIdx.x % pieces, lanes = blockDim.x / pieces;
     const uint64_t pos = a.positions[t];
+    for (uint32_t w = threadIdx.x; w < hd / 2; w += blockDim.x)
+    {
+        // half turns in [-1, 1)
+        const float half_turns = __ll2float_rn((long long)(pos * a.turns[w])) * 0x1p-63f;
+        float s, c;
+        sincospif(half_turns, &s, &c);
+        table[w] = make_float2(c, s);
+    }
+    __syncthreads();
     float cs[P], sn[P];
 #pragma unroll
     for (int i = 0; i < P; ++i)
-    {
-        // half turns in [-1, 1)
-        const float half_turns = __ll2float_rn((long long)(pos * a.turns[piece * P + i])) * 0x1p-63f;
-        sincospif(half_turns, &sn[i], &cs[i]);
-    }
+        cs[i] = table[piece * P + i].x, sn[i] = table[piece * P + i].y;
     const uint32_t H = a.heads, K = a.kv.kv_heads, rows = H + 2 * K, off = piece * E;
     const uint64_t cache = page * a.kv.page_stride + row * a.kv.row_stride + off;
-    for (uint32_t r = blockIdx.y * lanes + threadIdx.x / pieces; r < rows; r += gridDim.y * lanes)
+    const uint32_t step = gridDim.y * lanes;
+    for (uint32_t r0 = blockIdx.y * lanes + threadIdx.x / pieces; r0 < rows; r0 += kRopeAhead * step)
     {
-        const T *src;
-        T *dst;
-        if (r < H)
-        {
-            src = (const T *)a.q + t * a.q_stride + (uint64_t)r * hd + off;
-            dst = (T *)a.q_out + t * a.q_out_stride + (uint64_t)r * hd + off;
-        }
-        else if (r < H + K)
-        {
-            src = (const T *)a.k + t * a.k_stride + (uint64_t)(r - H) * hd + off;
-            dst = (T *)a.kv.k + cache + (r - H) * a.kv.head_stride;
-        }
-        else
-        {
-            src = (const T *)a.v + t * a.v_stride + (uint64_t)(r - H - K) * hd + off;
-            dst = (T *)a.kv.v + cache + (r - H - K) * a.kv.head_stride;
-        }
-        uint4 x = *reinterpret_cast<const uint4 *>(src);
-        if (r < H + K)
-        {
-            float2 p[P];
-            Piece<T>::load(x, p);
+        uint4 x[kRopeAhead];
 #pragma unroll
-            for (int i = 0; i < P; ++i)
-                p[i] = make_float2(cs[i] * p[i].x - sn[i] * p[i].y, sn[i] * p[i].x + cs[i] * p[i].y);
-            x = Piece<T>::store(p);
+        for (uint32_t u = 0; u < kRopeAhead; ++u)
+        {
+            const uint32_t r = r0 + u * step;
+            if (r >= rows)
+                break;
+            const T *src = r < H       ? (const T *)a.q + t * a.q_stride + (uint64_t)r * hd
+                           : r < H + K ? (const T *)a.k + t * a.k_stride + (uint64_t)(r - H) * hd
+                                       : (const T *)a.v + t * a.v_stride + (uint64_t)(r - H - K) * hd;
+            x[u] = *reinterpret_cast<const uint4 *>(src + off);
         }
-        *reinterpret_cast<uint4 *>(dst) = x;
+#pragma unroll
+        for (uint32_t u = 0; u < kRopeAhead; ++u)
+        {
+            const uint32_t r = r0 + u * step;
+            if (r >= rows)
+                break;
+            if (r < H + K)
+            {
+                float2 p[P];
+                Piece<T>::load(x[u], p);
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+                    p[i] = make_float2(cs[i] * p[i].x - sn[i] * p[i].y, sn[i] * p[i].x + cs[i] * p[i].y);
+                x[u] = Piece<T>::store(p);
+            }
+            T *dst = r < H       ? (T *)a.q_out + t * a.q_out_stride + (uint64_t)r * hd + off
+                     : r < H + K ? (T *)a.kv.k + cache + (r - H) * a.kv.head_stride
+                                 : (T *)a.kv.v + cache + (r - H - K) * a.kv.head_stride;
+            *reinterpret_cast<uint4 *>(dst) = x[u];
+        }
     }
 }
 
@@ -170,9 +183,10 @@ extern "C" vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged
     for (uint32_t w = 0; w < hd / 2; ++w, f *= ratio)
         a.turns[w] = (uint64_t)f;
     const uint32_t pieces = hd * es / 16, threads = kRopeThreads / pieces * pieces, lanes = threads / pieces;
-    // few tokens: several blocks share a token's rows so that the call reaches about two blocks an SM
+    // Blocks of a token: so many that a thread has one batch of rows in flight (2048 tokens of 120 heads: 2 blocks
+    // a token 24.6 us, one 25.9), and of few tokens more, until the call reaches about two blocks an SM.
     const uint32_t passes = (heads + 2 * kv->kv_heads + lanes - 1) / lanes;
-    uint32_t shares = 1;
+    uint32_t shares = (passes + kRopeAhead - 1) / kRopeAhead;
     while (shares < passes && (uint64_t)n_tokens * shares < 2u * (uint32_t)sms)
         ++shares;
     const dim3 grid(n_tokens, shares);

@@ -10,7 +10,8 @@
 // The floor is the words in and out (8 bytes a token and 20 a sequence), microseconds at most: the calls
 // are bound by the latency of one launch and of a few dependent loads.
 //
-// One thread-block cluster does a call. Every CTA sums all sequences itself (they are few; a scan split over CTAs
+// One thread-block cluster does a call (but for the slots of many tokens, which a second kernel spreads over the GPU).
+// Every CTA sums all sequences itself (they are few; a scan split over CTAs
 // would need an exchange more) into shared memory, then takes its share of the tokens, pages and
 // sequences, found by binary search in the sums, so one long prompt among many short ones spreads
 // evenly. The cluster barrier between the last read and the first write is what makes all-or-nothing
@@ -50,6 +51,10 @@ namespace
 constexpr uint32_t kMaxSeqs = 16384; // three words a sequence in shared memory
 constexpr uint32_t kTabThreads = 512;
 constexpr uint32_t kMaxCluster = 8;
+// Most tokens whose slots the cluster writes itself. More go to a second kernel over the whole GPU: a release and an
+// append of 131072 tokens in 512 sequences took 23.9 us with one cluster for all, and take 13.5 this way.
+constexpr uint32_t kTokensHere = kMaxCluster * kTabThreads;
+constexpr uint32_t kSlotThreads = 256;
 
 struct AppendArgs
 {
@@ -121,6 +126,7 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_append(const AppendArgs a
     const uint32_t n = a.t.n_seqs, R = a.t.page_rows, tid = threadIdx.x;
     const uint32_t rank = cg::this_cluster().block_rank(), size = cg::this_cluster().num_blocks();
     uint32_t *starts = sm, *first = sm + n + 1, *len = first + n + 1; // [n + 1], [n + 1], [n]
+    const uint32_t nf = *a.n_free;
     if (tid == 0)
         err = 0;
     __syncthreads();
@@ -137,7 +143,6 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_append(const AppendArgs a
     }
     uint64_t tokens, pages;
     block_sums(tok, pg, &tokens, &pages);
-    const uint32_t nf = *a.n_free;
     if (nf > a.t.n_pages || pages > nf)
         e |= VKLLM_B200_PAGED_NO_PAGES;
     if (tokens > a.max_tokens)
@@ -158,6 +163,7 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_append(const AppendArgs a
         if (tid == 0)
             starts[n] = (uint32_t)tokens, first[n] = (uint32_t)pages;
         // the ids that the call would use: pages off the list and partly filled pages that get more rows
+#pragma unroll 4
         for (uint32_t j = rank * kTabThreads + tid; j < pages; j += size * kTabThreads)
             e |= page_status(a.t.free_pages[nf - 1 - j], a.t.n_pages);
         __syncthreads();
@@ -178,6 +184,7 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_append(const AppendArgs a
         tokens = pages = 0;
         __syncthreads();
     }
+    asm volatile("griddepcontrol.launch_dependents;");
     const uint32_t g0 = rank * kTabThreads + tid, step = size * kTabThreads;
     if (g0 == 0)
     {
@@ -189,25 +196,86 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_append(const AppendArgs a
         a.starts[s] = starts[s];
         a.new_lens[s] = len[s] + (starts[s + 1] - starts[s]);
     }
+#pragma unroll 4
     for (uint32_t j = g0; j < pages; j += step)
     {
-        const uint32_t s = last_at_most(first, n, j);
-        a.t.table[s * a.t.stride + pages_of(len[s], R) + (j - first[s])] = a.t.free_pages[nf - 1 - j];
+        const uint32_t page = a.t.free_pages[nf - 1 - j], s = last_at_most(first, n, j);
+        a.t.table[s * a.t.stride + pages_of(len[s], R) + (j - first[s])] = page;
     }
-    for (uint64_t t = g0; t < a.max_tokens; t += step)
+    if (a.max_tokens > kTokensHere) // k_paged_slots
+        return;
+    for (uint32_t t = g0; t < a.max_tokens; t += step)
     {
         uint32_t slot = VKLLM_B200_NO_SLOT, pos = 0;
         if (t < tokens)
         {
-            const uint32_t s = last_at_most(starts, n, (uint32_t)t);
-            pos = len[s] + ((uint32_t)t - starts[s]);
-            const uint32_t c = pos / R, held = pages_of(len[s], R);
+            const uint32_t s = last_at_most(starts, n, t), held = pages_of(len[s], R);
+            pos = len[s] + (t - starts[s]);
+            const uint32_t c = pos / R;
             const uint32_t page = c < held ? a.t.table[s * a.t.stride + c] : a.t.free_pages[nf - 1 - (first[s] + (c - held))];
             slot = page * R + pos % R;
         }
         a.slots[t] = slot;
         a.positions[t] = pos;
     }
+}
+
+// Slots and positions of many tokens, from what k_paged_append left: runs of four per thread, which mostly share
+// their sequence, its search and its page.
+__global__ void __launch_bounds__(kSlotThreads) k_paged_slots(const AppendArgs a)
+{
+    extern __shared__ uint32_t starts[];
+    const uint32_t n = a.t.n_seqs, R = a.t.page_rows;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (uint32_t s = threadIdx.x; s <= n; s += kSlotThreads)
+        starts[s] = a.starts[s];
+    __syncthreads();
+    const uint32_t tokens = starts[n];
+    const uint64_t t0 = ((uint64_t)blockIdx.x * kSlotThreads + threadIdx.x) * 4;
+    if (t0 >= a.max_tokens)
+        return;
+    const uint32_t t = (uint32_t)t0;
+    uint32_t slot[4], pos[4];
+    uint32_t s = 0, p = 0, row = 0, c = 0, page = 0; // of the token: its sequence, position, row, column and page
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+    {
+        slot[i] = VKLLM_B200_NO_SLOT, pos[i] = 0;
+        if (t0 + i >= tokens)
+            continue;
+        bool fresh = i == 0 || t + i == starts[s + 1]; // another sequence, or another page
+        if (fresh)
+        {
+            if (i == 0)
+                s = last_at_most(starts, n, t);
+            else
+                do
+                    ++s;
+                while (t + i == starts[s + 1]);
+            p = a.new_lens[s] - (starts[s + 1] - (t + i)); // tokens end at the sequence's new end
+            c = p / R, row = p - c * R;
+        }
+        else
+        {
+            ++p, ++row;
+            if (row == R)
+                row = 0, ++c, fresh = true;
+        }
+        if (fresh)
+            page = a.t.table[s * a.t.stride + c];
+        slot[i] = page * R + row;
+        pos[i] = p;
+    }
+    if (t0 + 4 <= a.max_tokens && (((uintptr_t)a.slots | (uintptr_t)a.positions) & 15) == 0)
+    {
+        *reinterpret_cast<uint4 *>(a.slots + t) = make_uint4(slot[0], slot[1], slot[2], slot[3]);
+        *reinterpret_cast<uint4 *>(a.positions + t) = make_uint4(pos[0], pos[1], pos[2], pos[3]);
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+        if (t0 + i < a.max_tokens)
+            a.slots[t + i] = slot[i], a.positions[t + i] = pos[i];
 }
 
 __global__ void __launch_bounds__(kTabThreads) k_paged_release(const ReleaseArgs a)
@@ -217,7 +285,8 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_release(const ReleaseArgs
     __shared__ uint32_t err;
     const uint32_t n = a.t.n_seqs, R = a.t.page_rows, tid = threadIdx.x;
     const uint32_t rank = cg::this_cluster().block_rank(), size = cg::this_cluster().num_blocks();
-    uint32_t *first = sm, *len = sm + n + 1; // [n + 1], [n]: the length after the call
+    uint32_t *first = sm, *len = sm + n + 1; // [n + 1], [n]
+    const uint32_t nf = *a.n_free;
     if (tid == 0)
         err = 0;
     __syncthreads();
@@ -236,7 +305,6 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_release(const ReleaseArgs
     }
     uint64_t pages, total;
     block_sums(pg, unused, &pages, &total);
-    const uint32_t nf = *a.n_free;
     if ((uint64_t)nf + pages > a.t.n_pages)
         e |= VKLLM_B200_PAGED_TOO_MANY;
     if (e)
@@ -253,6 +321,7 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_release(const ReleaseArgs
         if (tid == 0)
             first[n] = (uint32_t)pages;
         __syncthreads();
+#pragma unroll 4
         for (uint32_t j = rank * kTabThreads + tid; j < pages; j += size * kTabThreads)
         {
             const uint32_t s = last_at_most(first, n, j);
@@ -272,6 +341,7 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_release(const ReleaseArgs
         *a.n_free_out = nf + (uint32_t)pages;
     for (uint32_t s = g0; s < n; s += step)
         a.new_lens[s] = ok && a.done[s] ? 0 : len[s];
+#pragma unroll 4
     for (uint32_t j = g0; j < pages; j += step)
     {
         const uint32_t s = last_at_most(first, n, j);
@@ -331,9 +401,28 @@ extern "C" vkllm_err_t vkllm_b200_paged_append(const struct vkllm_b200_paged_tab
     int dev = 0;
     _CHECK(check_device(t->table, nullptr, &dev));
     const AppendArgs a{*t, lens, n_new, n_free, new_lens, n_free_out, starts, slots, positions, max_tokens, status};
-    const uint64_t items = max_tokens > t->n_seqs ? max_tokens : t->n_seqs;
-    return launch_cluster(k_paged_append, a, cluster_for(items), (3 * (size_t)t->n_seqs + 2) * 4, dev,
-                          (cudaStream_t)stream);
+    const uint32_t here = max_tokens <= kTokensHere ? max_tokens : 0, items = here > t->n_seqs ? here : t->n_seqs;
+    cudaStream_t s = (cudaStream_t)stream;
+    _CHECK(launch_cluster(k_paged_append, a, here == max_tokens ? cluster_for(items) : kMaxCluster,
+                          (3 * (size_t)t->n_seqs + 2) * 4, dev, s));
+    if (here == max_tokens)
+        return VKLLM_ERR_OK;
+    const uint32_t smem = (t->n_seqs + 1) * 4;
+    if (smem > 48 * 1024)
+        VKB_CUDA(cudaFuncSetAttribute((const void *)k_paged_slots, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)((kMaxSeqs + 1) * 4)));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(((uint64_t)max_tokens + 4 * kSlotThreads - 1) / (4 * kSlotThreads)));
+    cfg.blockDim = dim3(kSlotThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; // its launch overlaps the first kernel
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    VKB_CUDA(cudaLaunchKernelEx(&cfg, k_paged_slots, a));
+    return VKLLM_ERR_OK;
 }
 
 extern "C" vkllm_err_t vkllm_b200_paged_release(const struct vkllm_b200_paged_table *t, const uint32_t *lens,
@@ -346,7 +435,8 @@ extern "C" vkllm_err_t vkllm_b200_paged_release(const struct vkllm_b200_paged_ta
     int dev = 0;
     _CHECK(check_device(t->table, nullptr, &dev));
     const ReleaseArgs a{*t, lens, done, n_free, new_lens, n_free_out, status};
-    return launch_cluster(k_paged_release, a, cluster_for(t->n_seqs), (2 * (size_t)t->n_seqs + 1) * 4, dev,
+    return launch_cluster(k_paged_release, a, cluster_for((uint64_t)t->n_seqs * 16), // the pages are not known here
+                           (2 * (size_t)t->n_seqs + 1) * 4, dev,
                           (cudaStream_t)stream);
 }
 
