@@ -4,18 +4,20 @@
 //   x = x - frequency * (times generated) - (generated ? presence : 0)
 //   x = x + the id's biases;  x = mask bit ? x : -infinity
 //
-// Every logit is read and written once (HBM bounds a large batch, latency a single row), but the
-// penalties and biases touch at most as many ids as the history and the lists are long. So two kernels:
+// Every logit is read and written once (HBM bounds a large batch, latency a few rows), but the
+// penalties and biases touch at most as many ids as the history and the lists are long. So there are two steps:
 //   k_logits_copy   streams the rows through, with the mask: out = mask bit ? x : -infinity. In place it writes masked
 //                   logits only, and without a mask it is not launched.
 //   k_logits_touch  one block per row: the touched ids with their counts and bias sums in a hash table in
 //                   shared memory, then x read, ruled, rounded once and written at those ids.
 // The second is the first one's programmatic dependent: it builds its tables while the first streams
 // and waits for it only before it touches the rows. The first's grid is resident at once for that
-// reason. (One kernel that counted the history in every piece of a row spent most of its time there:
-// 256 rows of 100003 fp16 logits with 1024 to 2048 ids of history, 62.9 us.)
+// reason. Few rows take one kernel, k_logits_touch<T, true>, whose blocks do both steps for a piece of a row.
 // Counts are integer atomics, and biases are added by one warp in the order of the list: the result does
 // not depend on the order of arrival.
+// 256 rows of 100003 fp16 logits with 1024 to 2048 ids of history, all rules (107 MB): 31.0 us, of which the first kernel
+// alone takes 23 and a plain copy of as much 19. What is left is the second one's scattered reads and writes, 1000
+// ids a row. (All in one kernel of pieces: 62.9 us with counts in arrays over the piece, 44 with hash tables.)
 #include <atomic>
 #include <cmath>
 
@@ -28,15 +30,15 @@ namespace
 {
 
 // 16-byte vectors that a thread has in flight, and CTAs per SM: 48 KB of loads, and registers left for a block of the
-// other kernel. (256 rows of 100003 fp16 logits, all rules: 31.9 us; 4 vectors x 4 or 5 CTAs 33.8, 33.0; two items in
-// flight a thread 34.1.)
+// other kernel. (256 rows of 100003 fp16 logits, all rules, when the whole took 31.9 us: 4 vectors x 4 or 5 CTAs 33.8, 33.0; two
+// items in flight a thread 34.1.)
 constexpr uint32_t kCopyThreads = 256, kCopyVecs = 2, kCopyCtas = 6;
-constexpr uint32_t kTouchThreads = 512, kHistoryThreads = kTouchThreads - 32; // the last warp sums the biases
+constexpr uint32_t kTouchThreads = 512; // of a row, or half as many where rows share an SM (see launch)
 // Slots of the hash table, 16 bytes each; it takes lists of up to 3/4 as many ids (with repeats), longer ones
 // go over ranges of the vocabulary instead. The small table lets more rows share an SM.
 constexpr uint32_t kSlotsSmall = 4096, kSlotsLarge = 8192;
 constexpr uint32_t kNoId = 0xffffffffu; // not an id: vocab < 2^31
-constexpr uint32_t kSeen = 0x80000000u; // in the prompt; the bits below count the times generated
+constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u; // in the prompt; in the biases; the bits below: times generated
 
 struct RuleArgs
 {
@@ -167,14 +169,17 @@ template <typename T> __global__ void __launch_bounds__(kCopyThreads) k_logits_c
     }
 }
 
-template <typename T> __global__ void __launch_bounds__(kTouchThreads, 4) k_logits_touch(const RuleArgs a)
+// The touched ids: of a row (one block each), or with PIECE of one chunk of a row, which the block streams through
+// itself before.
+template <typename T, bool PIECE> __global__ void __launch_bounds__(kTouchThreads, 4) k_logits_touch(const RuleArgs a)
 {
     extern __shared__ uint32_t sm[];
     uint32_t *key = sm, *count = sm + a.slots;
     float *bias = reinterpret_cast<float *>(sm + 2 * a.slots);
     uint32_t *list = sm + 3 * a.slots;
     __shared__ uint32_t listed;
-    const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+    const uint32_t row = PIECE ? blockIdx.y : blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+    const uint32_t threads = blockDim.x, historians = threads - 32; // the last warp sums the biases
     const uint32_t have = a.r.history ? (uint32_t)min((uint64_t)a.r.history_lens[row], a.r.history_stride) : 0;
     const uint32_t prompt = a.r.history && a.r.prompt_lens ? a.r.prompt_lens[row] : 0;
     const uint32_t *h = a.r.history + row * a.r.history_stride;
@@ -182,26 +187,39 @@ template <typename T> __global__ void __launch_bounds__(kTouchThreads, 4) k_logi
     const uint32_t biases = b1 > b0 ? b1 - b0 : 0;
     const float rep = a.r.repetition ? a.r.repetition[row] : 1.f, freq = a.r.frequency ? a.r.frequency[row] : 0.f,
                 pres = a.r.presence ? a.r.presence[row] : 0.f;
-    // Few enough ids: hashed, in a table of at least 4/3 their number. Else ranges of the vocabulary one after the
+    uint32_t id0 = 0, id1 = a.vocab; // the block's ids
+    if constexpr (PIECE)
+    {
+        CopyItem<T> item;
+        item.load(a, row, blockIdx.x);
+        if (a.x != a.y || a.r.mask)
+            item.store();
+        id0 = blockIdx.x * a.chunk > item.lead ? blockIdx.x * a.chunk - item.lead : 0;
+        id1 = item.stop > item.lead ? item.stop - item.lead : 0;
+    }
+    // Few enough entries: hashed, in a table of at least 4/3 their number. Else ranges of ids one after the
     // other, each id at its place.
-    const uint64_t ids = (uint64_t)have + biases;
-    const bool hashed = ids <= a.slots / 4 * 3;
+    const uint64_t entries = (uint64_t)have + biases;
+    const bool hashed = entries <= a.slots / 4 * 3;
     uint32_t slots = a.slots;
     if (hashed)
-        while (slots > 64 && slots / 2 >= ids + ids / 3)
+        while (slots > 64 && slots / 2 >= entries + entries / 3)
             slots /= 2;
-    bool waited = false;
-    for (uint32_t base = 0; base < (hashed ? 1u : a.vocab); base += a.slots)
+    bool waited = PIECE;
+    for (uint32_t base = id0, width; base < id1; base += width)
     {
-        for (uint32_t i = tid; i < slots; i += kTouchThreads)
+        width = hashed ? id1 - base : min(slots, id1 - base); // ids of this round: base .. base + width - 1
+        for (uint32_t i = tid; i < slots; i += threads)
             key[i] = kNoId, count[i] = 0, bias[i] = 0.f;
+        if (tid == 0)
+            listed = 0;
         __syncthreads();
         // the slot of an id, or kNoId where it has none
         auto place = [&](uint32_t id) {
-            if (id >= a.vocab)
+            if (id - base >= width)
                 return kNoId;
             if (!hashed)
-                return id - base < slots ? id - base : kNoId;
+                return id - base;
             uint32_t s = (id * 0x9E3779B1u) >> 8 & (slots - 1);
             for (;; s = (s + 1) & (slots - 1)) // ends: the table has more slots than ids
             {
@@ -212,24 +230,31 @@ template <typename T> __global__ void __launch_bounds__(kTouchThreads, 4) k_logi
                     return s;
             }
         };
-        if (tid < kHistoryThreads)
+        auto enlist = [&](uint32_t s, bool fresh) { // one count per warp: all lanes together
+            const uint32_t who = __ballot_sync(0xffffffffu, fresh);
+            uint32_t at = 0;
+            if (who && lane == 0)
+                at = atomicAdd(&listed, (uint32_t)__popc(who));
+            at = __shfl_sync(0xffffffffu, at, 0);
+            if (fresh)
+                list[at + __popc(who & ((1u << lane) - 1))] = s;
+        };
+        if (tid < historians)
         {
-            for (uint32_t i0 = tid; i0 < have; i0 += 4 * kHistoryThreads)
+            for (uint32_t i0 = tid - lane; i0 < have; i0 += 4 * historians) // (the whole warp together)
             {
                 uint32_t id[4];
 #pragma unroll
                 for (uint32_t u = 0; u < 4; ++u)
-                    id[u] = i0 + u * kHistoryThreads < have ? h[i0 + u * kHistoryThreads] : kNoId;
+                    id[u] = i0 + lane + u * historians < have ? h[i0 + lane + u * historians] : kNoId;
 #pragma unroll
                 for (uint32_t u = 0; u < 4; ++u)
                 {
                     const uint32_t s = place(id[u]);
-                    if (s == kNoId)
-                        continue;
-                    if (i0 + u * kHistoryThreads < prompt)
-                        atomicOr(&count[s], kSeen);
-                    else
-                        atomicAdd(&count[s], 1u);
+                    bool fresh = false; // the first to touch it
+                    if (s != kNoId)
+                        fresh = (i0 + lane + u * historians < prompt ? atomicOr(&count[s], kSeen) : atomicAdd(&count[s], 1u)) == 0;
+                    enlist(s, fresh);
                 }
             }
         }
@@ -243,6 +268,7 @@ template <typename T> __global__ void __launch_bounds__(kTouchThreads, 4) k_logi
                 const uint32_t s = place(id), peers = __match_any_sync(0xffffffffu, s);
                 const uint32_t turn = __popc(peers & ((1u << lane) - 1));
                 const uint32_t turns = __reduce_max_sync(0xffffffffu, s == kNoId ? 0u : turn);
+                enlist(s, s != kNoId && turn == 0 && atomicOr(&count[s], kBiased) == 0);
                 for (uint32_t k = 0; k <= turns; ++k)
                 {
                     if (turn == k && s != kNoId)
@@ -252,59 +278,64 @@ template <typename T> __global__ void __launch_bounds__(kTouchThreads, 4) k_logi
                 if (biases - b <= 32)
                     break;
             }
-        if (tid == 0)
-            listed = 0;
         __syncthreads();
-        // The touched ids that the mask allows, packed: what is left to do after the wait is one round of loads.
+        // ids that the mask forbids leave the list
         const uint32_t *mask = a.r.mask ? a.r.mask + row * a.r.mask_stride : nullptr;
-        for (uint32_t i0 = tid; i0 < slots; i0 += 4 * kTouchThreads)
-        {
-            uint32_t id[4], allowed[4];
-#pragma unroll
-            for (uint32_t u = 0; u < 4; ++u)
+        const uint32_t n = listed;
+        if (mask)
+            for (uint32_t i0 = tid; i0 < n; i0 += 4 * threads)
             {
-                const uint32_t i = i0 + u * kTouchThreads;
-                id[u] = kNoId;
-                if (i < slots && (count[i] != 0 || bias[i] != 0.f))
-                    id[u] = hashed ? key[i] : base + i;
-                allowed[u] = id[u] != kNoId ? (mask ? __ldg(mask + (id[u] >> 5)) : 0xffffffffu) : 0u;
-            }
+                uint32_t word[4];
 #pragma unroll
-            for (uint32_t u = 0; u < 4; ++u)
-                if ((allowed[u] >> (id[u] & 31)) & 1u)
-                    list[atomicAdd(&listed, 1u)] = i0 + u * kTouchThreads;
-        }
-        __syncthreads();
+                for (uint32_t u = 0; u < 4; ++u)
+                    if (i0 + u * threads < n)
+                    {
+                        const uint32_t s = list[i0 + u * threads];
+                        word[u] = __ldg(mask + ((hashed ? key[s] : base + s) >> 5));
+                    }
+#pragma unroll
+                for (uint32_t u = 0; u < 4; ++u)
+                    if (i0 + u * threads < n)
+                    {
+                        const uint32_t s = list[i0 + u * threads];
+                        if (!((word[u] >> ((hashed ? key[s] : base + s) & 31)) & 1u))
+                            list[i0 + u * threads] = kNoId;
+                    }
+            }
         if (!waited) // the rows are the first kernel's until it is done
             asm volatile("griddepcontrol.wait;" ::: "memory");
         waited = true;
-        // Out of place the logits are read back from the output, where the first kernel just put them: they are in
-        // L2, while the input's lines would be fetched from memory once more.
+        // A row's logits are read back from the output, where the first kernel just put them: they are in L2, while the
+        // input's lines would be fetched from memory once more. A piece's are still there from its own loads (in place
+        // as well: what the mask allows is as it was).
         T *y = (T *)a.y + row * a.y_stride;
-        const uint32_t n = listed;
-        for (uint32_t i0 = tid; i0 < n; i0 += 4 * kTouchThreads)
+        const T *in = PIECE ? (const T *)a.x + row * a.x_stride : y;
+        for (uint32_t i0 = tid; i0 < n; i0 += 4 * threads)
         {
             uint32_t id[4], s[4];
             T x[4];
 #pragma unroll
             for (uint32_t u = 0; u < 4; ++u)
-                if (i0 + u * kTouchThreads < n)
+            {
+                s[u] = i0 + u * threads < n ? list[i0 + u * threads] : kNoId;
+                if (s[u] != kNoId)
                 {
-                    s[u] = list[i0 + u * kTouchThreads];
                     id[u] = hashed ? key[s[u]] : base + s[u];
-                    x[u] = y[id[u]];
+                    x[u] = in[id[u]];
                 }
+            }
 #pragma unroll
             for (uint32_t u = 0; u < 4; ++u)
-                if (i0 + u * kTouchThreads < n)
+                if (s[u] != kNoId)
                 {
                     const uint32_t c = count[s[u]];
                     float v = to_f32<T>(x[u]);
-                    if (c)
+                    if (c != kBiased)
                     {
                         v = v > 0.f ? v / rep : v * rep;
-                        if (c != kSeen)
-                            v = v - freq * (float)(c & ~kSeen) - pres;
+                        const uint32_t times = c & ~(kSeen | kBiased);
+                        if (times)
+                            v = v - freq * (float)times - pres;
                     }
                     y[id[u]] = from_f32<T>(v + bias[s[u]]);
                 }
@@ -323,16 +354,28 @@ template <typename T> vkllm_err_t launch_rules(RuleArgs &a, int sms, int device,
     static std::atomic<bool> done[64]; // the kernels' attributes, set once a device (twice does no harm)
     if (device >= 64 || !done[device].load(std::memory_order_relaxed))
     {
-        VKB_CUDA(cudaFuncSetAttribute((const void *)k_logits_touch<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        VKB_CUDA(cudaFuncSetAttribute((const void *)k_logits_touch<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)(kSlotsLarge * 16)));
+        VKB_CUDA(cudaFuncSetAttribute((const void *)k_logits_touch<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)(kSlotsLarge * 16)));
         // an SM changes its split of L1 and shared memory only when it is idle: with the same split for both,
         // the second kernel's blocks can join the first one's
-        VKB_CUDA(cudaFuncSetAttribute((const void *)k_logits_touch<T>, cudaFuncAttributePreferredSharedMemoryCarveout,
+        VKB_CUDA(cudaFuncSetAttribute((const void *)k_logits_touch<T, false>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                       cudaSharedmemCarveoutMaxShared));
         VKB_CUDA(cudaFuncSetAttribute((const void *)k_logits_copy<T>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                       cudaSharedmemCarveoutMaxShared));
         if (device < 64)
             done[device].store(true, std::memory_order_relaxed);
+    }
+    // One kernel while its blocks run at once: each reads the whole history, but nothing waits for a second kernel.
+    // Of 32000 fp16 logits with up to 768 ids of history, 4 / 32 / 64 / 128 rows take 5.7 / 6.9 / 11.0 / 16.8 us in one
+    // kernel and 9.5 / 10.4 / 10.6 / 11.4 in two; of 32000 fp32 ones with up to 5000 ids, where the large table
+    // leaves an SM one block, 16 rows 24.6 and 16.5.
+    if (copy && touch && (uint64_t)a.rows * a.chunks <= (a.slots == kSlotsSmall ? 2 : 1) * (uint64_t)sms)
+    {
+        k_logits_touch<T, true><<<dim3(a.chunks, a.rows), kCopyThreads, a.slots * 16, s>>>(a);
+        VKB_CUDA(cudaGetLastError());
+        return VKLLM_ERR_OK;
     }
     if (copy)
     {
@@ -344,7 +387,7 @@ template <typename T> vkllm_err_t launch_rules(RuleArgs &a, int sms, int device,
         return VKLLM_ERR_OK;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.rows);
-    cfg.blockDim = dim3(kTouchThreads);
+    cfg.blockDim = dim3(a.rows <= (uint32_t)sms ? kTouchThreads : kTouchThreads / 2);
     cfg.dynamicSmemBytes = a.slots * 16;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -352,7 +395,7 @@ template <typename T> vkllm_err_t launch_rules(RuleArgs &a, int sms, int device,
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = copy ? 1 : 0; // alone it follows whatever is in the stream
-    VKB_CUDA(cudaLaunchKernelEx(&cfg, k_logits_touch<T>, a));
+    VKB_CUDA(cudaLaunchKernelEx(&cfg, k_logits_touch<T, false>, a));
     return VKLLM_ERR_OK;
 }
 
