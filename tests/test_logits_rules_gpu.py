@@ -107,7 +107,8 @@ def close(got, ref, tol, dtype):
 @pytest.mark.parametrize("rows,vocab,past,bias,pad", [(1, 1, 1, 1, 0), (1, 32000, 700, 8, 0), (3, 31, 40, 3, 2),
                                                       (5, 4097, 300, 40, 1), (2, 8192, 5000, 300, 8),
                                                       (64, 1003, 20, 2, 0), (7, 100003, 900, 33, 3),
-                                                      (3, 20011, 9000, 40, 1), (2, 40, 6144, 0, 0), (2, 9000, 6100, 70, 0)])
+                                                      (3, 20011, 9000, 40, 1), (2, 40, 6144, 0, 0), (2, 9000, 6100, 70, 0),
+                                                      (200, 5000, 60, 4, 0), (160, 4099, 4000, 3, 1)])
 def test_rules(vk, dtype, on, rows, vocab, past, bias, pad):
     import torch
 
@@ -162,6 +163,69 @@ def test_biases_of_one_id_add_in_the_order_of_the_list(vk):
     for v in values:
         want = np.float32(want + v)
     assert float(out[0, 13]) == float(want)
+
+
+def test_one_id_over_and_over(vk):
+    """A history of one repeated id, in the prompt and after it, that is also biased."""
+    import torch
+
+    c = case(3, 40000, 3000, 8, "f32")
+    c["history"][:], c["history_lens"][:] = 123, [3000, 2999, 1]
+    c["prompt_lens"][:] = [1000, 2999, 0]
+    c["bias_ids"][:] = 123
+    c["mask"][:] = 0xffffffff
+    x = torch.from_numpy(c["x"]).cuda()
+    out = torch.zeros_like(x)
+    assert run(vk, torch, c, ALL, "f32", x, out) == vk.OK
+    ref, tol = reference(c, ALL)
+    close(out.cpu().numpy().astype(np.float64), ref, tol, "f32")
+
+
+@pytest.mark.parametrize("rows", [2, 70])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_captured_and_replayed_with_new_tokens(vk, rows, in_place):
+    """One captured call (few rows: one kernel; more: two, the second launched early) replayed while the
+    history, its lengths and the logits change, as a decoding server's do."""
+    import torch
+
+    c = case(rows, 32000, 400, 21, "f16")
+    dev = {k: torch.from_numpy(c[k].view(np.int32) if c[k].dtype == np.uint32 else c[k]).cuda() for k in ALL}
+    r = vk.LogitRules(**{k: t.data_ptr() for k, t in dev.items()}, history_stride=c["history"].shape[1],
+                      mask_stride=c["mask"].shape[1])
+    x = torch.from_numpy(c["x"]).cuda()
+    out = x if in_place else torch.zeros_like(x)
+    fresh = x.clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x.copy_(fresh)
+        assert vk.lib().vkllm_b200_logits_apply(C.byref(r), x.data_ptr(), 32000, rows, 32000, vk.F16, out.data_ptr(), 32000,
+                                                torch.cuda.current_stream().cuda_stream) == vk.OK
+    rng = np.random.default_rng(4)
+    for _ in range(4):
+        c["x"] = (rng.standard_normal((rows, 32000)) * 5).astype(np.float16)
+        c["history_lens"] = np.minimum(c["history_lens"] + 1, 400).astype(np.uint32)
+        c["history"][np.arange(rows), c["history_lens"] - 1] = rng.integers(0, 32000, rows)
+        fresh.copy_(torch.from_numpy(c["x"]))
+        dev["history"].copy_(torch.from_numpy(c["history"].view(np.int32)))
+        dev["history_lens"].copy_(torch.from_numpy(c["history_lens"].view(np.int32)))
+        g.replay()
+        torch.cuda.synchronize()
+        ref, tol = reference(c, ALL)
+        close(out.cpu().numpy().astype(np.float64), ref, tol, "f16")
+
+
+def test_memory_that_is_not_the_devices_is_refused(vk):
+    import torch
+
+    c = case(1, 64, 4, 1, "f16")
+    dev = {k: torch.from_numpy(c[k].view(np.int32) if c[k].dtype == np.uint32 else c[k]).cuda() for k in ALL}
+    x = torch.from_numpy(c["x"]).cuda()
+    host = torch.zeros(4096, dtype=torch.float16).pin_memory().data_ptr()
+    for bad in ALL + ["logits", "out"]:
+        r = vk.LogitRules(**{k: host if k == bad else t.data_ptr() for k, t in dev.items()}, history_stride=7, mask_stride=3)
+        assert vk.lib().vkllm_b200_logits_apply(C.byref(r), host if bad == "logits" else x.data_ptr(), 64, 1, 64, vk.F16,
+                                                host if bad == "out" else x.data_ptr(), 64, None) == vk.ARGS, bad
 
 
 def test_infinities_and_no_numbers(vk):

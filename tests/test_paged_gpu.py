@@ -554,13 +554,58 @@ def test_attention_flags_bad_pages_and_lengths(vk, torch, dtype):
     assert bool((a.out[4:] == 7.5).all())
 
 
-def test_attention_refuses_memory_that_is_not_the_devices(vk, torch):
+def test_memory_that_is_not_the_devices_is_refused(vk, torch):
+    """Every array of every call in turn as pinned host memory: refused, and nothing runs."""
     a = Attend(vk, torch, [20], 2, 2, 64, 16, "f16")
-    host = torch.zeros(1 << 16, dtype=torch.float16).pin_memory()
-    a.kv.k = host.data_ptr()
-    assert a.call() == vk.ARGS
-    status = torch.zeros(1, dtype=torch.int32, device="cuda")
-    assert rope_call(vk, torch, a.kv, a.q, 2, 2, 64, a.d_lens, a.d_lens, 1, 0.0, a.out, status) == vk.ARGS
+    host = torch.zeros(1 << 16, dtype=torch.float16).pin_memory().data_ptr()
+    out0 = a.out.clone()
+    for name in ("k", "v"):
+        keep = getattr(a.kv, name)
+        setattr(a.kv, name, host)
+        assert a.call() == vk.ARGS, name
+        setattr(a.kv, name, keep)
+    s, kv, t, lib = stream(torch), C.byref(a.kv), C.byref(a.table), vk.lib()
+    dev, n = a.q.data_ptr(), 8
+    at = lambda i, k: host if i == k else dev  # noqa: E731
+    for k in range(5):
+        assert lib.vkllm_b200_paged_attention(kv, t, at(0, k), a.q.stride(0), 2, at(1, k), 0.1,
+                                              host if k == 2 else a.out.data_ptr(), a.out.stride(0),
+                                              host if k == 3 else a.ws.data_ptr(), a.ws.numel(), at(4, k), s) == vk.ARGS, k
+    for k in range(7):
+        assert lib.vkllm_b200_paged_rope_write(kv, at(0, k), 128, at(1, k), 128, at(2, k), 128, at(3, k), at(4, k), n, 2, 0.0,
+                                               host if k == 5 else a.out.data_ptr(), 128, at(6, k), s) == vk.ARGS, k
+    t2 = vk.PagedTable(a.d_tab.data_ptr(), a.d_tab.data_ptr(), 4, 1, 2, 16, 4)
+    for k in range(9):
+        assert lib.vkllm_b200_paged_append(C.byref(t2), *(at(i, k) for i in range(8)), 4, at(8, k), s) == vk.ARGS, k
+    for k in range(6):
+        assert lib.vkllm_b200_paged_release(C.byref(t2), *(at(i, k) for i in range(6)), s) == vk.ARGS, k
+    t2.free_pages = host
+    assert lib.vkllm_b200_paged_append(C.byref(t2), *[dev] * 8, 4, dev, s) == vk.ARGS
+    torch.cuda.synchronize()
+    assert torch.equal(a.out, out0)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_of_random_shapes(vk, torch, seed):
+    rng = np.random.default_rng(900 + seed)
+    HK, group = int(rng.integers(1, 9)), int(rng.choice([1, 2, 3, 5, 8, 12, 16, 20]))
+    hd = int(rng.integers(1, 33)) * 8
+    n, hi = int(rng.integers(1, 40)), int(2 ** rng.uniform(0, 11))
+    lens = [int(x) for x in rng.integers(0, hi + 1, n)]
+    a = Attend(vk, torch, lens, HK * group, HK, hd, int(rng.choice([1, 3, 16, 32, 100])), ["f16", "f32"][seed % 2],
+               LAYOUTS[int(rng.integers(0, 3))], seed=seed)
+    assert a.call() == vk.OK
+    a.check(f"{HK} x {group} heads of {hd}, {n} up to {hi}")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_of_sequences_that_share_pages(vk, torch, dtype):
+    """A common beginning held once: both tables name its pages."""
+    a = Attend(vk, torch, [100, 90, 70], 8, 2, 64, 16, dtype, seed=31, poison=False)
+    a.tab[1, :4], a.tab[2, :4] = a.tab[0, :4], a.tab[0, :4]
+    a.d_tab.copy_(i32(torch, a.tab))
+    assert a.call() == vk.OK
+    a.check()
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])

@@ -421,7 +421,11 @@ extern "C" vkllm_err_t vkllm_b200_logits_apply(const struct vkllm_b200_logit_rul
     _CHECK_ARGS(!rules->mask || (words(rules->mask) && rules->mask_stride >= ((uint64_t)vocab + 31) / 32));
     _CHECK_ARGS(rules->history_stride < (1ull << 40) && rules->mask_stride < (1ull << 40));
     int sms = 0, dev = 0;
-    _CHECK(check_device(logits, &sms, &dev));
+    const vkllm_b200_logit_rules &r = *rules;
+    _CHECK(check_device({logits, out, r.history, r.history ? r.prompt_lens : nullptr, r.history ? r.history_lens : nullptr, r.repetition,
+                         r.frequency, r.presence, r.bias_starts, r.bias_starts ? r.bias_ids : nullptr,
+                         r.bias_starts ? r.bias_values : nullptr, r.mask},
+                        &sms, &dev));
     // the longest history that fits the small table with 512 biases
     const uint32_t slots = !rules->history || rules->history_stride <= kSlotsSmall / 4 * 3 - 512 ? kSlotsSmall : kSlotsLarge;
     RuleArgs a{*rules, logits, out, logits_stride, out_stride, vocab, rows, slots, 0, 0};

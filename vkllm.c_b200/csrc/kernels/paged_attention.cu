@@ -60,24 +60,27 @@ struct PagedAttArgs
     float scale_log2; // scale * log2(e): the softmax runs in powers of two
     uint32_t *status;
     uint32_t *counters;
-    float *parts; // [2 * grid] parts of items: [gq][HP] O, then [gq] m, [gq] l
+    float *parts; // [2 * grid] parts of items: [gq][KD] O, then [gq] m, [gq] l
     uint32_t part_stride;
 };
 
 constexpr uint32_t kRound = 4; // queries that the join buffers take at a time
 
-template <typename T, int HP> struct Shape
+// KD: dimensions that are computed, head_dim rounded up; HP: those that a row in shared memory has room for, a power of
+// two, so that its 16-byte pieces can be swizzled.
+template <typename T, int KD> struct Shape
 {
+    static constexpr int HP = KD <= 64 ? 64 : KD <= 128 ? 128 : 256;
     static constexpr uint32_t kKeys = sizeof(T) == 2 ? 16 : 8;                  // keys of a slice
     static constexpr uint32_t kRow = HP * sizeof(T);                            // bytes of a row in shared memory
     static constexpr uint32_t kStage = 2 * kKeys * kRow;                        // K and V of a slice
-    static constexpr uint32_t kQBytes = sizeof(T) == 4 ? 8 * HP * 4 : 0;        // the queries (fp32 only)
-    static constexpr uint32_t kStages = sizeof(T) == 4 ? (HP == 64 ? 4 : 2) : HP == 64 ? 6 : 3;
-    static constexpr uint32_t kPitch = HP + 4;                                  // floats of a row of the join buffer
+    static constexpr uint32_t kQBytes = sizeof(T) == 4 ? 8 * KD * 4 : 0;        // the queries (fp32 only)
+    static constexpr uint32_t kStages = HP == 64 ? (sizeof(T) == 4 ? 3 : 4) : sizeof(T) == 4 ? 2 : 3;
+    static constexpr uint32_t kPitch = KD + 4;                                  // floats of a row of the join buffer
     static constexpr uint32_t kRing = kWarps * kStages * kStage;
     static constexpr uint32_t kJoin = kWarps * kRound * (kPitch + 2);           // floats of a join buffer: O, then m and l
     static constexpr uint32_t kSmem = kRing + kQBytes + 2 * kJoin * 4 + kWarps * kStages * 4;
-    static constexpr uint32_t kCtas = HP == 256 ? 1 : 2; // per SM
+    static constexpr uint32_t kCtas = HP == 256 ? 1 : HP == 64 ? 3 : 2; // per SM
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes)
@@ -117,6 +120,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
+}
+// Two fp32 FMAs in one instruction: c + a * b, element by element.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<const uint64_t *>(&a)), "l"(*reinterpret_cast<const uint64_t *>(&b)),
+          "l"(*reinterpret_cast<const uint64_t *>(&c)));
+    return *reinterpret_cast<const float2 *>(&d);
 }
 __device__ __forceinline__ float pow2(float x)
 {
@@ -177,17 +190,24 @@ struct Cursor
 };
 
 // The stream of one warp's slices: page ids one tile ahead, rows kStages - 1 tiles ahead.
-template <typename T, int HP, bool EXACT> struct Loader
+template <typename T, int KD, bool EXACT> struct Loader
 {
-    using S = Shape<T, HP>;
-    static constexpr uint32_t kPieces = S::kRow / 16;
+    using S = Shape<T, KD>;
+    static constexpr uint32_t kPieces = KD * sizeof(T) / 16;
     Cursor c;
     uint32_t end;  // units of the CTA's part
     uint32_t page; // of key `lane % kKeys` of the slice at c
     uint32_t ring; // shared address of the warp's ring
     uint32_t *valid; // [kStages] masks of the slice's keys that count
     uint32_t stage = 0, status = 0;
+    uint32_t pieces, row0, p0, drow, dp; // the copies of a lane: pieces of a row, its first one, from one to the next
 
+    __device__ __forceinline__ void set_pieces(const PagedAttArgs &a, uint32_t lane)
+    {
+        pieces = EXACT ? kPieces : a.kv.head_dim * (uint32_t)sizeof(T) / 16;
+        row0 = lane / pieces, p0 = lane % pieces;
+        drow = 32 / pieces, dp = 32 % pieces;
+    }
     __device__ __forceinline__ uint32_t key(uint32_t warp, uint32_t lane) const
     {
         return (c.tile * kWarps + warp) * S::kKeys + lane % S::kKeys;
@@ -227,10 +247,8 @@ template <typename T, int HP, bool EXACT> struct Loader
             if (mask)
             {
                 const uint32_t base = ring + stage * S::kStage;
-                const uint32_t pieces = EXACT ? kPieces : a.kv.head_dim * (uint32_t)sizeof(T) / 16;
-                uint32_t row = lane / pieces, p = lane % pieces;
-                const uint32_t drow = 32 / pieces, dp = 32 % pieces;
-                constexpr uint32_t kMost = S::kKeys * kPieces / 32;
+                uint32_t row = row0, p = p0;
+                constexpr uint32_t kMost = S::kKeys * kPieces / 32; // (a whole number for every KD)
 #pragma unroll
                 for (uint32_t i = 0; i < kMost; ++i)
                 {
@@ -246,7 +264,7 @@ template <typename T, int HP, bool EXACT> struct Loader
                         cp_async16(dst + S::kKeys * S::kRow, (const T *)a.kv.v + off, bytes);
                     }
                     row += drow, p += dp;
-                    if ((!EXACT || kPieces > 32) && p >= pieces)
+                    if ((!EXACT || 32 % kPieces != 0) && p >= pieces)
                         p -= pieces, ++row;
                 }
             }
@@ -261,12 +279,12 @@ template <typename T, int HP, bool EXACT> struct Loader
 };
 
 // What a warp keeps of an item: statistics and outputs of its keys, for 8 NQ queries.
-template <int HP, int NQ, bool EXACT> struct HalfCore
+template <int KD, int NQ, bool EXACT> struct HalfCore
 {
     using T = __half;
-    using S = Shape<T, HP>;
+    using S = Shape<T, KD>;
     static constexpr int kQueries = 8 * NQ;
-    static constexpr int kK = HP / 16;
+    static constexpr int kK = KD / 16;
     uint32_t qf[NQ][kK][2]; // Q^T as the B operand
     float o[NQ][kK][4], m[NQ][2], l[NQ][2];
 
@@ -405,14 +423,14 @@ template <int HP, int NQ, bool EXACT> struct HalfCore
 
 // fp32: 8 keys of a slice; lane = (part << 3) | key computes a quarter of that key's dot products (the
 // 16-byte pieces p with p % 4 == part); for the outputs a lane owns the pieces lane % kP, lane % kP + 32 ...
-template <int HP, int NQ, bool EXACT> struct FloatCore
+template <int KD, int NQ, bool EXACT> struct FloatCore
 {
     using T = float;
-    using S = Shape<T, HP>;
+    using S = Shape<T, KD>;
     static constexpr int kQueries = NQ;
-    static constexpr int kP = HP / 4;                       // pieces of a row
+    static constexpr int kP = S::HP / 4;                    // pieces that a row has room for
     static constexpr int kOwn = kP > 32 ? kP / 32 : 1;      // pieces that a lane owns
-    static constexpr int kHalves = kP < 32 ? 32 / kP : 1;   // lane groups that share the keys (HP = 64: 2)
+    static constexpr int kHalves = kP < 32 ? 32 / kP : 1;   // lane groups that share the keys (KD = 64: 2)
     float4 o[NQ][kOwn];
     float m[NQ], l[NQ];
 
@@ -422,8 +440,8 @@ template <int HP, int NQ, bool EXACT> struct FloatCore
         // the CTA's warps are at the same item here: each loads its share of the queries
         const uint32_t hd = a.kv.head_dim, warp = threadIdx.x >> 5;
         for (uint32_t i = warp; i < NQ; i += kWarps)
-            for (uint32_t d = lane; d < HP; d += 32)
-                qs[i * HP + d] = i < nq && d < hd ? ((const T *)a.q)[seq * a.q_stride + (uint64_t)(head0 + i) * hd + d] : 0.f;
+            for (uint32_t d = lane; d < KD; d += 32)
+                qs[i * KD + d] = i < nq && d < hd ? ((const T *)a.q)[seq * a.q_stride + (uint64_t)(head0 + i) * hd + d] : 0.f;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
@@ -444,30 +462,27 @@ template <int HP, int NQ, bool EXACT> struct FloatCore
         const float4 *V = K + S::kKeys * kP;
         const uint32_t key = lane & 7, part = lane >> 3;
         // every query's dot product in two chains (even and odd elements), all queries side by side
-        float d[NQ][2];
+        float2 d[NQ];
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
-            d[i][0] = d[i][1] = 0.f;
-        const uint32_t quads = EXACT ? kP / 4 : (a.kv.head_dim / 4 + 3) / 4; // quads of pieces that hold something
+            d[i] = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int j = 0; j < kP / 4; ++j)
+        for (int j = 0; j < KD / 16; ++j)
         {
-            if (!EXACT && j >= quads)
-                break;
             const float4 k = K[key * kP + ((4 * j + part) ^ key)];
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
             {
-                const float4 q = reinterpret_cast<const float4 *>(qs + i * HP)[4 * j + part];
-                d[i][0] = fmaf(q.x, k.x, d[i][0]), d[i][1] = fmaf(q.y, k.y, d[i][1]);
-                d[i][0] = fmaf(q.z, k.z, d[i][0]), d[i][1] = fmaf(q.w, k.w, d[i][1]);
+                const float4 q = reinterpret_cast<const float4 *>(qs + i * KD)[4 * j + part];
+                d[i] = fma2(make_float2(q.x, q.y), make_float2(k.x, k.y), d[i]);
+                d[i] = fma2(make_float2(q.z, q.w), make_float2(k.z, k.w), d[i]);
             }
         }
         const bool in = (mask >> key) & 1u;
         float p[NQ], mx[NQ];
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
-            p[i] = d[i][0] + d[i][1];
+            p[i] = d[i].x + d[i].y;
 #pragma unroll
         for (int x = 8; x < 32; x <<= 1)
 #pragma unroll
@@ -515,8 +530,9 @@ template <int HP, int NQ, bool EXACT> struct FloatCore
 #pragma unroll
                 for (int k = 0; k < kOwn; ++k)
                 {
-                    o[i][k].x = fmaf(w, v[k].x, o[i][k].x), o[i][k].y = fmaf(w, v[k].y, o[i][k].y);
-                    o[i][k].z = fmaf(w, v[k].z, o[i][k].z), o[i][k].w = fmaf(w, v[k].w, o[i][k].w);
+                    const float2 lo = fma2(make_float2(w, w), make_float2(v[k].x, v[k].y), make_float2(o[i][k].x, o[i][k].y));
+                    const float2 hi = fma2(make_float2(w, w), make_float2(v[k].z, v[k].w), make_float2(o[i][k].z, o[i][k].w));
+                    o[i][k] = make_float4(lo.x, lo.y, hi.x, hi.y);
                 }
             }
         }
@@ -545,7 +561,7 @@ template <int HP, int NQ, bool EXACT> struct FloatCore
                     v.x += __shfl_xor_sync(0xffffffffu, v.x, 16), v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
                     v.z += __shfl_xor_sync(0xffffffffu, v.z, 16), v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
                 }
-                if (kHalves == 1 || lane < kP)
+                if (lane % kP + 32 * k < KD / 4 && (kHalves == 1 || lane < kP))
                     *reinterpret_cast<float4 *>(os + q * S::kPitch + 4 * (lane % kP + 32 * k)) = v;
             }
         }
@@ -569,14 +585,14 @@ __device__ __forceinline__ void add_scaled(float4 &o, float f, const float4 &v)
 }
 
 // A join buffer, joined over the warps: queries q0 .. q0 + n - 1 of the item (at most kRound), to the output or to a part.
-template <typename T, int HP>
+template <typename T, int KD>
 __device__ __forceinline__ void join_warps(const PagedAttArgs &a, const float *os, const float *ml, uint32_t n,
                                            uint32_t q0, uint32_t seq, uint32_t head0, float *part)
 {
-    using S = Shape<T, HP>;
-    for (uint32_t i = threadIdx.x; i < n * (HP / 4); i += kThreads)
+    using S = Shape<T, KD>;
+    for (uint32_t i = threadIdx.x; i < n * (KD / 4); i += kThreads)
     {
-        const uint32_t q = i / (HP / 4), d = i % (HP / 4) * 4;
+        const uint32_t q = i / (KD / 4), d = i % (KD / 4) * 4;
         float mx = -INFINITY;
 #pragma unroll
         for (uint32_t w = 0; w < kWarps; ++w)
@@ -593,9 +609,9 @@ __device__ __forceinline__ void join_warps(const PagedAttArgs &a, const float *o
         }
         if (part)
         {
-            *reinterpret_cast<float4 *>(part + (q0 + q) * HP + d) = o;
+            *reinterpret_cast<float4 *>(part + (q0 + q) * KD + d) = o;
             if (d == 0)
-                part[a.gq * HP + q0 + q] = mx, part[a.gq * (HP + 1) + q0 + q] = l;
+                part[a.gq * KD + q0 + q] = mx, part[a.gq * (KD + 1) + q0 + q] = l;
         }
         else if (d < a.kv.head_dim)
             store_out<T>(a, seq, head0 + q0 + q, d, o, l);
@@ -612,11 +628,11 @@ __device__ __forceinline__ float *part_of(const PagedAttArgs &a, uint32_t c, boo
 // the end of a CTA's work: so every thread takes 4 elements of a query with the statistics of their parts on its
 // own, 16 parts in flight, and where the item has too few elements to fill the CTA, and parts enough, groups of
 // threads take every `groups`-th part and meet in shared memory.
-template <typename T, int HP>
+template <typename T, int KD>
 __device__ __noinline__ void join_parts(const PagedAttArgs &a, uint32_t c0, uint32_t c1, float *sm, uint32_t nq,
                                         uint32_t seq, uint32_t head0)
 {
-    constexpr uint32_t kCols = HP / 4, kAhead = 16;
+    constexpr uint32_t kCols = KD / 4, kAhead = 16;
     const uint32_t cols = nq * kCols, np = c1 - c0 + 1;
     const uint32_t groups = np > kAhead && cols < kThreads ? kThreads / cols : 1;
     const uint32_t group = groups > 1 ? threadIdx.x / cols : 0;
@@ -637,8 +653,8 @@ __device__ __noinline__ void join_parts(const PagedAttArgs &a, uint32_t c0, uint
                 if (p > c1)
                     continue;
                 const float *src = part_of(a, p, p == c0);
-                m[u] = __ldcg(src + a.gq * HP + q), pl[u] = __ldcg(src + a.gq * (HP + 1) + q);
-                v[u] = __ldcg(reinterpret_cast<const float4 *>(src + q * HP + d));
+                m[u] = __ldcg(src + a.gq * KD + q), pl[u] = __ldcg(src + a.gq * (KD + 1) + q);
+                v[u] = __ldcg(reinterpret_cast<const float4 *>(src + q * KD + d));
             }
 #pragma unroll
             for (uint32_t u = 0; u < kAhead; ++u)
@@ -686,11 +702,11 @@ __device__ __noinline__ void join_parts(const PagedAttArgs &a, uint32_t c0, uint
     __syncthreads();
 }
 
-template <template <int, int, bool> class Kind, typename T, int HP, int NQ, bool EXACT>
-__global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attention(const __grid_constant__ PagedAttArgs a)
+template <template <int, int, bool> class Kind, typename T, int KD, int NQ, bool EXACT>
+__global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attention(const __grid_constant__ PagedAttArgs a)
 {
-    using S = Shape<T, HP>;
-    using Core = Kind<HP, NQ, EXACT>;
+    using S = Shape<T, KD>;
+    using Core = Kind<KD, NQ, EXACT>;
     constexpr uint32_t kTile = kWarps * S::kKeys;
     constexpr int kRounds = (Core::kQueries + kRound - 1) / kRound;
     extern __shared__ __align__(128) unsigned char sm[];
@@ -788,11 +804,12 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
     __syncthreads();
 
     Cursor c = first;
-    Loader<T, HP, EXACT> ld;
+    Loader<T, KD, EXACT> ld;
     ld.c = c;
     ld.end = end;
     ld.ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * S::kStages * S::kStage;
     ld.valid = valid + warp * S::kStages;
+    ld.set_pieces(a, lane);
     ld.lookup(a, warp, lane);
 #pragma unroll
     for (uint32_t i = 0; i + 1 < S::kStages; ++i)
@@ -828,7 +845,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
             float *os = join + buffer * S::kJoin, *ml = os + kWarps * kRound * S::kPitch;
             core.deposit(r, nq, os + warp * kRound * S::kPitch, ml + warp * kRound * 2, lane);
             __syncthreads();
-            join_warps<T, HP>(a, os, ml, min(nq - r * kRound, kRound), r * kRound, c.seq, head0, part);
+            join_warps<T, KD>(a, os, ml, min(nq - r * kRound, kRound), r * kRound, c.seq, head0, part);
             buffer ^= 1;
         }
         if (!whole)
@@ -848,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
             {
                 if (tid == 0)
                     a.counters[c0] = 0; // ready for the next call
-                join_parts<T, HP>(a, c0, c1, join, nq, c.seq, head0);
+                join_parts<T, KD>(a, c0, c1, join, nq, c.seq, head0);
             }
         }
         c.tile = from + n - 1;
@@ -859,11 +876,11 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP>::kCtas) k_paged_attenti
         atomicOr(a.status, ld.status);
 }
 
-template <template <int, int, bool> class Kind, typename T, int HP, int NQ, bool EXACT>
+template <template <int, int, bool> class Kind, typename T, int KD, int NQ, bool EXACT>
 vkllm_err_t launch(PagedAttArgs &a, int sms, int device, cudaStream_t s)
 {
-    using S = Shape<T, HP>;
-    auto kernel = k_paged_attention<Kind, T, HP, NQ, EXACT>;
+    using S = Shape<T, KD>;
+    auto kernel = k_paged_attention<Kind, T, KD, NQ, EXACT>;
     static std::atomic<bool> done[64]; // the attribute of this kernel, set once a device (twice does no harm)
     if (device >= 64 || !done[device].load(std::memory_order_relaxed))
     {
@@ -871,7 +888,7 @@ vkllm_err_t launch(PagedAttArgs &a, int sms, int device, cudaStream_t s)
         if (device < 64)
             done[device].store(true, std::memory_order_relaxed);
     }
-    a.part_stride = a.gq * (HP + 2);
+    a.part_stride = a.gq * (KD + 2);
     a.part_stride = (a.part_stride + 3) / 4 * 4;
     // most CTAs that can have work, that the counters and the workspace serve, and that the GPU holds at once
     const uint32_t tiles = (uint32_t)((a.cap + (uint64_t)kWarps * S::kKeys - 1) / (kWarps * S::kKeys));
@@ -887,21 +904,21 @@ vkllm_err_t launch(PagedAttArgs &a, int sms, int device, cudaStream_t s)
     return VKLLM_ERR_OK;
 }
 
-template <template <int, int, bool> class Kind, typename T, int HP, int NQ>
+template <template <int, int, bool> class Kind, typename T, int KD, int NQ>
 vkllm_err_t launch_exact(PagedAttArgs &a, int sms, int device, cudaStream_t s)
 {
-    return a.kv.head_dim == HP ? launch<Kind, T, HP, NQ, true>(a, sms, device, s)
-                               : launch<Kind, T, HP, NQ, false>(a, sms, device, s);
+    return a.kv.head_dim == KD ? launch<Kind, T, KD, NQ, true>(a, sms, device, s)
+                               : launch<Kind, T, KD, NQ, false>(a, sms, device, s);
 }
 
-template <int HP> vkllm_err_t launch_head(PagedAttArgs &a, int sms, int device, cudaStream_t s)
+template <int KD> vkllm_err_t launch_head(PagedAttArgs &a, int sms, int device, cudaStream_t s)
 {
     if (a.kv.dtype == vkllm_dtype_float16)
-        return a.gq <= 8 ? launch_exact<HalfCore, __half, HP, 1>(a, sms, device, s)
-                         : launch_exact<HalfCore, __half, HP, 2>(a, sms, device, s);
-    return a.gq == 1   ? launch_exact<FloatCore, float, HP, 1>(a, sms, device, s)
-           : a.gq <= 4 ? launch_exact<FloatCore, float, HP, 4>(a, sms, device, s)
-                       : launch_exact<FloatCore, float, HP, 8>(a, sms, device, s);
+        return a.gq <= 8 ? launch_exact<HalfCore, __half, KD, 1>(a, sms, device, s)
+                         : launch_exact<HalfCore, __half, KD, 2>(a, sms, device, s);
+    return a.gq == 1   ? launch_exact<FloatCore, float, KD, 1>(a, sms, device, s)
+           : a.gq <= 4 ? launch_exact<FloatCore, float, KD, 4>(a, sms, device, s)
+                       : launch_exact<FloatCore, float, KD, 8>(a, sms, device, s);
 }
 
 } // namespace
@@ -923,7 +940,7 @@ extern "C" vkllm_err_t vkllm_b200_paged_attention(const struct vkllm_b200_paged_
     _CHECK_ARGS(words(lens) && words(status));
     _CHECK_ARGS(workspace && aligned_to(workspace, 16) && workspace_bytes >= VKLLM_B200_PAGED_WORKSPACE_BYTES);
     int sms = 0, dev = 0;
-    _CHECK(check_device(kv->k, &sms, &dev));
+    _CHECK(check_device({kv->k, kv->v, t->table, q, lens, out, workspace, status}, &sms, &dev));
     PagedAttArgs a;
     a.kv = *kv;
     a.table = t->table, a.table_stride = t->stride, a.n_seqs = t->n_seqs;
@@ -938,9 +955,10 @@ extern "C" vkllm_err_t vkllm_b200_paged_attention(const struct vkllm_b200_paged_
     a.status = status;
     a.counters = (uint32_t *)workspace;
     a.parts = (float *)((char *)workspace + kCounters * 4);
-    if (kv->head_dim <= 64)
-        return launch_head<64>(a, sms, dev, (cudaStream_t)stream);
-    if (kv->head_dim <= 128)
-        return launch_head<128>(a, sms, dev, (cudaStream_t)stream);
-    return launch_head<256>(a, sms, dev, (cudaStream_t)stream);
+    cudaStream_t s = (cudaStream_t)stream;
+    return kv->head_dim <= 64    ? launch_head<64>(a, sms, dev, s)
+           : kv->head_dim <= 96  ? launch_head<96>(a, sms, dev, s)
+           : kv->head_dim <= 128 ? launch_head<128>(a, sms, dev, s)
+           : kv->head_dim <= 192 ? launch_head<192>(a, sms, dev, s)
+                                 : launch_head<256>(a, sms, dev, s);
 }

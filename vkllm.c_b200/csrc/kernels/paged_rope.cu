@@ -170,7 +170,7 @@ extern "C" vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged
     _CHECK_ARGS(q != q_out || q_stride == q_out_stride);
     _CHECK_ARGS(words(positions) && words(slots) && words(status));
     int sms = 0;
-    _CHECK(check_device(kv->k, &sms, nullptr));
+    _CHECK(check_device({kv->k, kv->v, q, k, v, positions, slots, q_out, status}, &sms, nullptr));
     RopeArgs a;
     a.kv = *kv;
     a.q = q, a.k = k, a.v = v, a.q_out = q_out;

@@ -27,16 +27,21 @@
 namespace vkb
 {
 
-vkllm_err_t check_device(const void *p, int *sms, int *device)
+vkllm_err_t check_device(std::initializer_list<const void *> arrays, int *sms, int *device)
 {
-    cudaPointerAttributes a;
     int dev = 0;
     VKB_CUDA(cudaGetDevice(&dev));
-    VKB_CUDA(cudaPointerGetAttributes(&a, p));
-    if ((a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) || a.device != dev)
+    for (const void *p : arrays)
     {
-        log_error("an array is not memory of the current device (%d)", dev);
-        return VKLLM_ERR_ARGS;
+        cudaPointerAttributes a;
+        if (!p)
+            continue;
+        VKB_CUDA(cudaPointerGetAttributes(&a, p));
+        if ((a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) || a.device != dev)
+        {
+            log_error("an array is not memory of the current device (%d)", dev);
+            return VKLLM_ERR_ARGS;
+        }
     }
     if (device)
         *device = dev;
@@ -399,7 +404,9 @@ extern "C" vkllm_err_t vkllm_b200_paged_append(const struct vkllm_b200_paged_tab
                 words(status));
     _CHECK_ARGS(max_tokens == 0 || (words(slots) && words(positions)));
     int dev = 0;
-    _CHECK(check_device(t->table, nullptr, &dev));
+    _CHECK(check_device({t->table, t->free_pages, lens, n_new, n_free, new_lens, n_free_out, starts,
+                         max_tokens ? slots : nullptr, max_tokens ? positions : nullptr, status},
+                        nullptr, &dev));
     const AppendArgs a{*t, lens, n_new, n_free, new_lens, n_free_out, starts, slots, positions, max_tokens, status};
     const uint32_t here = max_tokens <= kTokensHere ? max_tokens : 0, items = here > t->n_seqs ? here : t->n_seqs;
     cudaStream_t s = (cudaStream_t)stream;
@@ -433,7 +440,7 @@ extern "C" vkllm_err_t vkllm_b200_paged_release(const struct vkllm_b200_paged_ta
     _CHECK_ARGS(table_fits(t) && words(t->free_pages) && t->n_seqs <= kMaxSeqs);
     _CHECK_ARGS(words(lens) && words(done) && words(n_free) && words(new_lens) && words(n_free_out) && words(status));
     int dev = 0;
-    _CHECK(check_device(t->table, nullptr, &dev));
+    _CHECK(check_device({t->table, t->free_pages, lens, done, n_free, new_lens, n_free_out, status}, nullptr, &dev));
     const ReleaseArgs a{*t, lens, done, n_free, new_lens, n_free_out, status};
     return launch_cluster(k_paged_release, a, cluster_for((uint64_t)t->n_seqs * 16), // the pages are not known here
                            (2 * (size_t)t->n_seqs + 1) * 4, dev,
