@@ -1,18 +1,22 @@
-/* Serving operators over a paged KV cache: page tables and slot maps built on the GPU, RoPE with the key and value rows written
- * into the pages, attention of one new token per sequence over them, and penalties, biases and grammar masks on the logits. None has
- * a counterpart in the reference, whose KV cache is one contiguous tensor per layer
- * (src/models/vkllm_kvcache.c) and whose token choice is a plain argmax.
+/* Serving operators over a paged KV cache: page tables and slot maps built on the GPU, RoPE with the
+ * key and value rows written into the pages, attention of one new token per sequence over them, and
+ * penalties, biases and grammar masks on the logits. None has a counterpart in the reference, whose KV
+ * cache is one contiguous tensor per layer (src/models/vkllm_kvcache.c) and whose token choice is a
+ * plain argmax.
  *
- * A step of a server that batches requests runs, per step: vkllm_b200_paged_release for sequences that
- * ended, vkllm_b200_paged_append; then per layer vkllm_b200_paged_rope_write and
- * vkllm_b200_paged_attention; then vkllm_b200_logits_apply before the argmax.
+ * A step of a server that batches requests runs vkllm_b200_paged_release for the sequences that ended
+ * and vkllm_b200_paged_append for the new tokens; then per layer vkllm_b200_paged_rope_write and
+ * vkllm_b200_paged_attention; then vkllm_b200_logits_apply before VKLLM_OP_ARG_MAX.
  *
- * Common to all: arrays are device memory of the device that is current at the call (structs and
- * vkllm_b200_paged_check's arrays are host memory); the work is enqueued on `stream` (a cudaStream_t, NULL = the legacy default
- * stream) and nothing waits; nothing is allocated, so every call can be captured into a CUDA graph.
- * VKLLM_ERR_ARGS: an argument does not fit, nothing was enqueued. VKLLM_ERR_VULKAN: a CUDA error.
- * Values in device memory that do not fit are found by the kernels: they set bits of the device word
- * *status (zeroed by the caller, only ever OR-ed into) and never read or write outside the arrays. */
+ * Common to all: arrays are device (or managed) memory of the device that is current at the call, which
+ * also owns `stream`; the structs, and the arrays of vkllm_b200_paged_check, are host memory. The work is
+ * enqueued on `stream` (a cudaStream_t, NULL = the legacy default stream) and nothing waits; nothing is
+ * allocated, so every call can be captured into a CUDA graph, whose replays read the arrays anew.
+ * VKLLM_ERR_ARGS: an argument does not fit (a pointer that is not the current device's among them),
+ * nothing was enqueued. VKLLM_ERR_VULKAN: a CUDA error.
+ * Lengths, counts, page ids and slots in device memory that do not fit are found by the kernels: they
+ * set bits of the device word *status (zeroed by the caller, only ever OR-ed into) and lead to no access
+ * outside the arrays. */
 #ifndef VKLLM_B200_PAGED_H
 #define VKLLM_B200_PAGED_H
 
@@ -37,6 +41,8 @@ enum
     VKLLM_B200_PAGED_NO_PAGES = 4,  /* append: more pages wanted than free (or *n_free > n_pages) */
     VKLLM_B200_PAGED_TOO_MANY = 8,  /* append: more new tokens than max_tokens; release: more pages than n_pages */
     VKLLM_B200_PAGED_BAD_SLOT = 16, /* rope_write: a slot >= n_pages * page_rows other than NO_SLOT */
+    VKLLM_B200_PAGED_BAD_WORKSPACE = 32, /* attention: the workspace was not zero at first, or two calls
+                                          * used it at the same time; rows of out are missing */
 };
 
 /* The page table of a batch of sequence slots. Row s of a sequence's cache is row s % page_rows of page
@@ -44,7 +50,7 @@ enum
 struct vkllm_b200_paged_table
 {
     uint32_t *table;      /* device, [n_seqs] rows of cols page ids */
-    uint32_t *free_pages; /* device, n_pages entries: a stack, *n_free ids from the bottom; attention needs none (NULL) */
+    uint32_t *free_pages; /* device, n_pages entries: a stack of *n_free ids; attention needs none (NULL) */
     uint64_t stride;      /* entries from one sequence's row to the next, >= cols */
     uint32_t n_seqs, cols, page_rows, n_pages;
 };
@@ -57,14 +63,15 @@ struct vkllm_b200_paged_kv
 {
     void *k, *v; /* device, 16-byte aligned */
     uint64_t page_stride, head_stride, row_stride; /* multiples of 16 bytes */
-    uint32_t n_pages, page_rows, kv_heads, head_dim; /* head_dim * element size a multiple of 16, head_dim <= 256 */
+    uint32_t n_pages, page_rows, kv_heads;
+    uint32_t head_dim; /* <= 256, head_dim * element size a multiple of 16 */
     uint32_t dtype;    /* vkllm_dtype_float16 or vkllm_dtype_float32: of the pools, q, k, v and out */
     uint32_t reserved; /* 0 */
 };
 
-/* Host only: checks host copies of a table (`table`, `free_pages` and the other pointers in host
- * memory) as the kernels do, and that no page is held twice. `n_free` ids of free_pages are looked at (0: free_pages may be NULL). Returns
- * VKLLM_ERR_OK or VKLLM_ERR_ARGS with *status (may be NULL) set to the bits above and *bad_seq (may be
+/* Host only: checks host copies of a table (all pointers in host memory) as the kernels do, and that no
+ * page is held twice. `n_free` ids of free_pages are looked at (0: free_pages may be NULL). Returns
+ * VKLLM_ERR_OK, or VKLLM_ERR_ARGS with *status (may be NULL) set to the bits above and *bad_seq (may be
  * NULL) to the first sequence at fault, n_seqs when it is the free list. */
 extern vkllm_err_t vkllm_b200_paged_check(const struct vkllm_b200_paged_table *t, const uint32_t *lens, uint32_t n_free,
                                           uint32_t *status, uint32_t *bad_seq);
@@ -93,13 +100,15 @@ extern vkllm_err_t vkllm_b200_paged_release(const struct vkllm_b200_paged_table 
                                             uint32_t *n_free_out, uint32_t *status, void *stream);
 
 /* RoPE of new tokens and their rows of the cache: q_out = rotated q, key row = rotated k, value row = v,
- * with the pairs and angles of VKLLM_OP_ROPE (elements 2w and 2w + 1 turned by positions[t] * rope_base^(-2w / head_dim);
- * src/shaders/vkllm_rope.comp), the angle reduced exactly at every position.
+ * with the pairs and angles of VKLLM_OP_ROPE (elements 2w and 2w + 1 turned by positions[t] *
+ * rope_base^(-2w / head_dim); src/shaders/vkllm_rope.comp), exact at far positions too.
  *   q [n_tokens] rows of heads * head_dim, k and v of kv_heads * head_dim, q_out as q; row strides in
  *   elements, multiples of 16 bytes, pointers 16-byte aligned: q, k and v may be parts of one row.
- *   heads a multiple of kv_heads; rope_base > 1 (<= 0: 10000). q_out may be q (same stride); it must not overlap otherwise.
+ *   heads a multiple of kv_heads; rope_base > 1 (<= 0: 10000). q_out may be q (same stride); it must not
+ *   overlap q, k or v otherwise.
  * A token whose slot is VKLLM_B200_NO_SLOT leaves the cache and its q_out row as they were; so does a
- * slot outside the pool, which sets VKLLM_B200_PAGED_BAD_SLOT. The other slots must differ. n_tokens may be 0. */
+ * slot outside the pool, which sets VKLLM_B200_PAGED_BAD_SLOT. The other slots must differ. n_tokens may
+ * be 0. */
 extern vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged_kv *kv, const void *q, uint64_t q_stride,
                                                const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
                                                const uint32_t *positions, const uint32_t *slots, uint32_t n_tokens,
@@ -120,8 +129,9 @@ extern vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged_kv 
  *   workspace  16-byte aligned, VKLLM_B200_PAGED_WORKSPACE_BYTES, zero before its first use; every call
  *          leaves it ready for the next. Calls (and replays of captured calls) that may run at the same
  *          time need a workspace each.
- * A length past cols * page_rows is cut to it and a page id >= n_pages has no keys; both set *status. Scores, softmax and sums are fp32; t->free_pages is not used. The same inputs give the same
- * bits on the same device. */
+ * A length past cols * page_rows is cut to it and a page id >= n_pages has no keys; both set *status.
+ * Sequences may share pages. Scores, softmax and sums are fp32. The same inputs give the same bits on
+ * the same device. n_seqs <= 65535. */
 extern vkllm_err_t vkllm_b200_paged_attention(const struct vkllm_b200_paged_kv *kv,
                                               const struct vkllm_b200_paged_table *t, const void *q, uint64_t q_stride,
                                               uint32_t heads, const uint32_t *lens, float scale, void *out,
@@ -137,7 +147,8 @@ struct vkllm_b200_logit_rules
     const float *repetition;      /* [rows], > 0: x / r where x > 0, else x * r, for ids in the history */
     const float *frequency;       /* [rows]: x - frequency * (times generated) */
     const float *presence;        /* [rows]: x - presence for ids generated at least once */
-    const uint32_t *bias_starts;  /* [rows + 1]: row r's biases are entries bias_starts[r] .. bias_starts[r + 1] */
+    const uint32_t *bias_starts;  /* [rows + 1], ascending: row r's biases are entries bias_starts[r] up to
+                                   * bias_starts[r + 1] of the two arrays, which must be as long */
     const uint32_t *bias_ids;     /* x + value; an id listed twice gets both, in the order of the list */
     const float *bias_values;
     const uint32_t *mask;         /* bit id % 32 of word id / 32 of a row: 0 makes the logit -infinity */
@@ -146,8 +157,8 @@ struct vkllm_b200_logit_rules
 
 /* out = logits under the rules, in the order of the struct (repetition, frequency and presence, biases,
  * mask), in fp32 and rounded once. logits and out are rows of `vocab` elements of `dtype`
- * (vkllm_dtype_float16 or vkllm_dtype_float32), strides in elements; out may be logits (same stride) and must
- * not overlap otherwise. Ids >= vocab in the history and the biases are ignored. A mask that leaves a
+ * (vkllm_dtype_float16 or vkllm_dtype_float32), strides in elements; out may be logits (same stride) and
+ * must not overlap otherwise. Ids >= vocab in the history and the biases are ignored. A mask that leaves a
  * row nothing gives a row of -infinity. rows <= 65535. */
 extern vkllm_err_t vkllm_b200_logits_apply(const struct vkllm_b200_logit_rules *rules, const void *logits,
                                            uint64_t logits_stride, uint32_t rows, uint32_t vocab, uint32_t dtype,

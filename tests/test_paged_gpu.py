@@ -608,6 +608,70 @@ def test_attention_of_sequences_that_share_pages(vk, torch, dtype):
     a.check()
 
 
+def test_attention_says_when_its_workspace_was_not_zero(vk, torch):
+    a = Attend(vk, torch, [40000], 8, 2, 64, 16, "f16")
+    a.ws.fill_(255)
+    assert a.call() == vk.OK
+    torch.cuda.synchronize()
+    assert int(a.status) == vk.PAGED_BAD_WORKSPACE
+    a.ws.zero_()
+    a.status.zero_()
+    assert a.call() == vk.OK
+    a.check()
+
+
+FIRST_CALLS = """
+import ctypes as C, sys
+sys.path[:0] = [{pkg!r}]
+import torch, vkllm_b200 as vk
+z = lambda *s, t=torch.int32: torch.zeros(s, dtype=t, device="cuda")
+lib, R, n = vk.lib(), 16, 2
+table, free, lens, count, new, starts, slots, pos, st, done = (z(n, 4), torch.arange(8, device="cuda", dtype=torch.int32),
+    z(n), z(1) + 8, z(n) + 20, z(n + 1), z(5000), z(5000), z(1), z(n))
+k, v = z(8, 2, R, 64, t=torch.float16), z(8, 2, R, 64, t=torch.float16)
+qkv = torch.randn(5000, 512, device="cuda").half()
+q, out = torch.zeros(5000, 256, device="cuda").half(), z(n, 256, t=torch.float16)
+ws = z(vk.PAGED_WORKSPACE_BYTES, t=torch.uint8)
+x, hist, hl = torch.randn(70, 32000, device="cuda").half(), z(70, 8), z(70) + 8
+y = torch.zeros_like(x)
+t = vk.PagedTable(table.data_ptr(), free.data_ptr(), 4, n, 4, R, 8)
+kv = vk.PagedKV(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), 64, 8, R, 2, 64, vk.F16, 0)
+rep = torch.ones(70, device="cuda") * 2
+rules = vk.LogitRules(history=hist.data_ptr(), history_lens=hl.data_ptr(), repetition=rep.data_ptr(), history_stride=8)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream().cuda_stream
+    p = lambda a: a.data_ptr()
+    assert lib.vkllm_b200_paged_release(C.byref(t), p(lens), p(done), p(count), p(lens), p(count), p(st), s) == vk.OK
+    assert lib.vkllm_b200_paged_append(C.byref(t), p(lens), p(new), p(count), p(lens), p(count), p(starts), p(slots), p(pos),
+                                       5000, p(st), s) == vk.OK
+    assert lib.vkllm_b200_paged_rope_write(C.byref(kv), p(qkv), 512, p(qkv) + 512, 512, p(qkv) + 768, 512, p(pos), p(slots), 5000,
+                                           4, 0.0, p(q), 256, p(st), s) == vk.OK
+    assert lib.vkllm_b200_paged_attention(C.byref(kv), C.byref(t), p(q), 256, 4, p(lens), 0.125, p(out), 256, p(ws), ws.numel(),
+                                          p(st), s) == vk.OK
+    assert lib.vkllm_b200_logits_apply(C.byref(rules), p(x), 32000, 70, 32000, vk.F16, p(y), 32000, s) == vk.OK
+g.replay()
+torch.cuda.synchronize()
+assert int(st) == 0 and lens.tolist() == [20, 20] and int(count) == 4 and slots[39:41].tolist()[1] == -1
+assert bool((y[:, 1:] == x[:, 1:]).all()) and bool((out != 0).any())
+w = torch.where(x[:, 0] > 0, x[:, 0] / 2, x[:, 0] * 2)
+assert bool((y[:, 0] == w).all())
+print("first calls ok")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured(vk, torch):
+    """Nothing has to run before the capture: no allocation, no lazy set-up that a capture forbids."""
+    import os
+    import subprocess
+    import sys
+
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "vkllm.c_b200")
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(pkg=pkg)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "first calls ok" in r.stdout, r.stderr[-2000:]
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_attention_captured_and_replayed_on_two_streams(vk, torch, dtype):
     """Two captured calls with a workspace each, replayed at the same time many times over, give the bits of

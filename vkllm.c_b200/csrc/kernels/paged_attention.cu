@@ -857,7 +857,10 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
             if (tid == 0)
             {
                 __threadfence(); // the part, which the barrier made this thread's to publish, before the count
-                last_one = atomicAdd(a.counters + c0, 1u) == c1 - c0;
+                const uint32_t came = atomicAdd(a.counters + c0, 1u);
+                last_one = came == c1 - c0;
+                if (came > c1 - c0)
+                    atomicOr(a.status, (uint32_t)VKLLM_B200_PAGED_BAD_WORKSPACE);
                 __threadfence();
             }
             __syncthreads();

@@ -116,7 +116,7 @@ _lib = None
 
 # include/vkllm_b200_paged.h
 NO_SLOT = 0xffffffff
-PAGED_BAD_PAGE, PAGED_TOO_LONG, PAGED_NO_PAGES, PAGED_TOO_MANY, PAGED_BAD_SLOT = 1, 2, 4, 8, 16
+PAGED_BAD_PAGE, PAGED_TOO_LONG, PAGED_NO_PAGES, PAGED_TOO_MANY, PAGED_BAD_SLOT, PAGED_BAD_WORKSPACE = 1, 2, 4, 8, 16, 32
 PAGED_WORKSPACE_BYTES = 16 << 20
 
 # name -> (restype, argtypes)
