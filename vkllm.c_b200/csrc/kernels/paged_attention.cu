@@ -41,6 +41,7 @@ constexpr uint32_t kCounters = 1024;      // words at the start of the workspace
 // Lengths on the line: a tile, and what an item costs beside its tiles (its queries read, its warps joined).
 constexpr uint32_t kTileUnits = 4, kItemUnits = 6;
 constexpr uint32_t kMinUnits = 2 * kTileUnits + kItemUnits; // least part of a CTA: an item of two tiles
+constexpr uint32_t kNoPage = 0xffffffffu;
 constexpr float kWeightShift = 15.f;      // weights are at most 2^15, below fp16's 65504
 
 struct PagedAttArgs
@@ -53,6 +54,8 @@ struct PagedAttArgs
     const void *q;
     void *out;
     uint64_t q_stride, out_stride;
+    uint64_t page_bytes, head_bytes, row_bytes; // strides of the pools
+    uint64_t page_magic; // ceil(2^64 / page_rows): its product with a key's number has the page's column above bit 64; 0: one row
     const uint32_t *lens;
     uint32_t group;  // queries that share a key head
     uint32_t qtiles; // tiles of these queries
@@ -157,6 +160,12 @@ __host__ __device__ __forceinline__ uint32_t item_units(uint32_t tiles)
     return tiles ? tiles * kTileUnits + kItemUnits : 0;
 }
 
+// a / b; places on the line mostly fit 32 bits, whose division takes a tenth of the time.
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b)
+{
+    return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
+}
+
 // A place in the line of tiles: tile `tile` of `tiles` of item (seq, hq), hq = key head * qtiles + query tile, `unit`
 // units behind the start of the CTA's part.
 struct Cursor
@@ -189,28 +198,31 @@ struct Cursor
     }
 };
 
-// The stream of one warp's slices: page ids one tile ahead, rows kStages - 1 tiles ahead.
+// The stream of one warp's slices: page ids one tile ahead, rows kStages - 1 tiles ahead. A warp issues a few hundred
+// instructions for a tile, with no other warp to hide their latency behind in a short call, so what can be worked out before is.
 template <typename T, int KD, bool EXACT> struct Loader
 {
     using S = Shape<T, KD>;
     static constexpr uint32_t kPieces = KD * sizeof(T) / 16;
+    static constexpr bool kFixed = EXACT && 32 % kPieces == 0; // a lane copies the same piece of every row that it copies
     Cursor c;
-    uint32_t end;  // units of the CTA's part
-    uint32_t page; // of key `lane % kKeys` of the slice at c
-    uint32_t ring; // shared address of the warp's ring
-    uint32_t *valid; // [kStages] masks of the slice's keys that count
+    uint32_t end;       // units of the CTA's part
+    uint32_t page, row; // of key `lane % kKeys` of the slice at c, and its row in the page
+    uint64_t head;      // bytes from a page's start to the item's key head
+    uint32_t ring;      // shared address of the warp's ring
+    uint32_t *valid;    // [kStages] masks of the slice's keys that count
     uint32_t stage = 0, status = 0;
     uint32_t pieces, row0, p0, drow, dp; // the copies of a lane: pieces of a row, its first one, from one to the next
+    const char *k, *v;                   // the pools (at the lane's piece where that is fixed)
 
-    __device__ __forceinline__ void set_pieces(const PagedAttArgs &a, uint32_t lane)
+    __device__ __forceinline__ void begin(const PagedAttArgs &a, uint32_t warp, uint32_t lane)
     {
         pieces = EXACT ? kPieces : a.kv.head_dim * (uint32_t)sizeof(T) / 16;
         row0 = lane / pieces, p0 = lane % pieces;
         drow = 32 / pieces, dp = 32 % pieces;
-    }
-    __device__ __forceinline__ uint32_t key(uint32_t warp, uint32_t lane) const
-    {
-        return (c.tile * kWarps + warp) * S::kKeys + lane % S::kKeys;
+        k = (const char *)a.kv.k + (kFixed ? p0 * 16 : 0), v = (const char *)a.kv.v + (kFixed ? p0 * 16 : 0);
+        lookup(a, warp, lane);
+        new_item(a, lane);
     }
     __device__ __forceinline__ bool more(const PagedAttArgs &a) const
     {
@@ -218,15 +230,27 @@ template <typename T, int KD, bool EXACT> struct Loader
     }
     __device__ __forceinline__ void lookup(const PagedAttArgs &a, uint32_t warp, uint32_t lane)
     {
-        const uint32_t k = key(warp, lane);
-        page = more(a) && k < c.len ? __ldg(a.table + c.seq * a.table_stride + k / a.kv.page_rows) : 0xffffffffu;
+        const uint32_t key = (c.tile * kWarps + warp) * S::kKeys + lane % S::kKeys;
+        const uint32_t col = a.page_magic ? (uint32_t)__umul64hi(key, a.page_magic) : key;
+        row = key - col * a.kv.page_rows;
+        page = kNoPage; // behind the end
+        if (more(a) && key < c.len)
+        {
+            page = __ldg(a.table + c.seq * a.table_stride + col);
+            if (page == kNoPage) // (n_pages is below it)
+                page = kNoPage - 1;
+        }
     }
-    __device__ __forceinline__ void prefetch_queries(const PagedAttArgs &a, uint32_t lane) const
+    // At an item's first tile: where its keys lie, and its queries, which will be wanted, on their way to L1.
+    __device__ __forceinline__ void new_item(const PagedAttArgs &a, uint32_t lane)
     {
-        const uint32_t qt = c.hq % a.qtiles, nq = min(a.gq, a.group - qt * a.gq);
-        const char *q = (const char *)((const T *)a.q + c.seq * a.q_stride +
-                                       (uint64_t)(c.hq / a.qtiles * a.group + qt * a.gq) * a.kv.head_dim);
-        for (uint32_t b = lane * 128; b < nq * a.kv.head_dim * (uint32_t)sizeof(T); b += 32 * 128)
+        uint32_t kh = c.hq, qt = 0;
+        if (a.qtiles > 1)
+            kh = c.hq / a.qtiles, qt = c.hq - kh * a.qtiles;
+        head = kh * a.head_bytes;
+        const uint32_t nq = min(a.gq, a.group - qt * a.gq);
+        const char *q = (const char *)((const T *)a.q + c.seq * a.q_stride + (uint64_t)(kh * a.group + qt * a.gq) * a.kv.head_dim);
+        for (uint32_t b = lane * 128; more(a) && b < nq * a.kv.head_dim * (uint32_t)sizeof(T); b += 32 * 128)
             asm volatile("prefetch.global.L1 [%0];" ::"l"(q + b));
     }
     // Issues the slice at c as one group of copies (an empty one behind the end) and moves on.
@@ -234,44 +258,60 @@ template <typename T, int KD, bool EXACT> struct Loader
     {
         if (more(a))
         {
-            const uint32_t k = key(warp, lane);
-            bool ok = k < c.len;
-            if (ok && page >= a.kv.n_pages)
-                ok = false, status |= VKLLM_B200_PAGED_BAD_PAGE;
-            const uint64_t at = ok ? page * a.kv.page_stride + (c.hq / a.qtiles) * a.kv.head_stride +
-                                         (k % a.kv.page_rows) * a.kv.row_stride
-                                   : 0;
+            const bool ok = page < a.kv.n_pages;
+            if (!ok && page != kNoPage)
+                status |= VKLLM_B200_PAGED_BAD_PAGE;
+            const uint64_t at = ok ? page * a.page_bytes + head + row * a.row_bytes : 0;
             const uint32_t mask = __ballot_sync(0xffffffffu, ok) & ((1u << S::kKeys) - 1);
             if (lane == 0)
                 valid[stage] = mask;
             if (mask)
             {
                 const uint32_t base = ring + stage * S::kStage;
-                uint32_t row = row0, p = p0;
                 constexpr uint32_t kMost = S::kKeys * kPieces / 32; // (a whole number for every KD)
-#pragma unroll
-                for (uint32_t i = 0; i < kMost; ++i)
+                if constexpr (kFixed)
                 {
-                    if (!EXACT && i * 32 >= S::kKeys * pieces)
-                        break;
-                    const uint32_t r = row % S::kKeys; // row < kKeys for every copy that is made
-                    const uint64_t off = __shfl_sync(0xffffffffu, at, r) + p * (16 / sizeof(T));
-                    const uint32_t bytes = (mask >> r) & 1u ? 16u : 0u;
-                    if (EXACT || row < S::kKeys)
+                    // row r = row0 + i * drow with row0 < drow, both powers of two: the swizzle splits in two
+                    constexpr uint32_t kRows = 32 / kPieces;
+                    const uint32_t lane_dst = base + row0 * S::kRow + (p0 ^ row0) * 16;
+#pragma unroll
+                    for (uint32_t i = 0; i < kMost; ++i)
                     {
-                        const uint32_t dst = base + r * S::kRow + ((p ^ (r & 7)) * 16);
-                        cp_async16(dst, (const T *)a.kv.k + off, bytes);
-                        cp_async16(dst + S::kKeys * S::kRow, (const T *)a.kv.v + off, bytes);
+                        const uint32_t r = row0 + i * kRows;
+                        const uint64_t off = __shfl_sync(0xffffffffu, at, r);
+                        const uint32_t bytes = (mask >> r) & 1u ? 16u : 0u;
+                        const uint32_t dst = (lane_dst ^ ((i * kRows & 7) * 16)) + i * kRows * S::kRow;
+                        cp_async16(dst, k + off, bytes);
+                        cp_async16(dst + S::kKeys * S::kRow, v + off, bytes);
                     }
-                    row += drow, p += dp;
-                    if ((!EXACT || 32 % kPieces != 0) && p >= pieces)
-                        p -= pieces, ++row;
+                }
+                else
+                {
+                    uint32_t r0 = row0, p = p0;
+#pragma unroll
+                    for (uint32_t i = 0; i < kMost; ++i)
+                    {
+                        if (!EXACT && i * 32 >= S::kKeys * pieces)
+                            break;
+                        const uint32_t r = r0 % S::kKeys; // r0 < kKeys for every copy that is made
+                        const uint64_t off = __shfl_sync(0xffffffffu, at, r) + p * 16;
+                        const uint32_t bytes = (mask >> r) & 1u ? 16u : 0u;
+                        if (EXACT || r0 < S::kKeys)
+                        {
+                            const uint32_t dst = base + r * S::kRow + ((p ^ (r & 7)) * 16);
+                            cp_async16(dst, k + off, bytes);
+                            cp_async16(dst + S::kKeys * S::kRow, v + off, bytes);
+                        }
+                        r0 += drow, p += dp;
+                        if (p >= pieces)
+                            p -= pieces, ++r0;
+                    }
                 }
             }
             c.next(a, items, kWarps * S::kKeys);
             lookup(a, warp, lane);
-            if (c.tile == 0 && more(a)) // a new item ahead: its queries will be wanted
-                prefetch_queries(a, lane);
+            if (c.tile == 0)
+                new_item(a, lane);
         }
         cp_commit();
         stage = stage + 1 == S::kStages ? 0 : stage + 1;
@@ -718,9 +758,16 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
     __shared__ uint32_t last_one;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t items = a.kv.kv_heads * a.qtiles; // of a sequence
-    if (!EXACT) // the pieces behind head_dim are never loaded: they have to be zeros, not whatever was there
-        for (uint32_t i = tid; i < S::kRing / 16; i += kThreads)
-            reinterpret_cast<uint4 *>(sm)[i] = make_uint4(0, 0, 0, 0);
+    if (!EXACT)
+    {
+        // the pieces of a key behind head_dim are never loaded: they have to be zeros, not whatever was there
+        const uint32_t have = a.kv.head_dim * (uint32_t)sizeof(T) / 16, gap = KD * (uint32_t)sizeof(T) / 16 - have;
+        for (uint32_t i = tid; i < kWarps * S::kStages * S::kKeys * gap; i += kThreads)
+        {
+            const uint32_t row = i / gap, r = row % S::kKeys, p = have + i % gap;
+            *reinterpret_cast<uint4 *>(sm + row / S::kKeys * S::kStage + r * S::kRow + (p ^ (r & 7)) * 16) = make_uint4(0, 0, 0, 0);
+        }
+    }
 
     // This CTA's part of the line: every thread sums a run of sequences, the one in whose run the part
     // begins finds its place. On the way, sequences without keys get their zeros (each from one CTA).
@@ -770,7 +817,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
             before += sums[w];
         total += sums[w];
     }
-    const uint64_t per = max((total + gridDim.x - 1) / gridDim.x, (uint64_t)kMinUnits);
+    const uint64_t per = max(quotient(total + gridDim.x - 1, gridDim.x), (uint64_t)kMinUnits);
     const uint64_t begin = blockIdx.x * per;
     if (begin >= total)
         return;
@@ -790,8 +837,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
             at += (uint64_t)units * items;
         }
         units = max(units, 1u);
-        c.hq = (uint32_t)((begin - at) / units);
-        const uint32_t x = (uint32_t)((begin - at) % units); // a tile is the CTA's in whose part its first unit lies
+        c.hq = (uint32_t)quotient(begin - at, units);
+        const uint32_t x = (uint32_t)(begin - at - (uint64_t)c.hq * units); // a tile is the CTA's in whose part its first unit lies
         c.tile = (x + kTileUnits - 1) / kTileUnits;
         c.unit = c.tile * kTileUnits - x;
         if (c.tile >= c.tiles)
@@ -809,9 +856,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
     ld.end = end;
     ld.ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * S::kStages * S::kStage;
     ld.valid = valid + warp * S::kStages;
-    ld.set_pieces(a, lane);
-    ld.lookup(a, warp, lane);
-#pragma unroll
+    ld.begin(a, warp, lane);
+#pragma unroll 1 // (a copy of the code for every round would only be fetched from memory once more)
     for (uint32_t i = 0; i + 1 < S::kStages; ++i)
         ld.issue(a, items, warp, lane);
 
@@ -821,7 +867,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
     {
         // one item, or this CTA's part of it
         const uint32_t from = c.tile, n = min(c.tiles - from, (end - c.unit + kTileUnits - 1) / kTileUnits);
-        const uint32_t qt = c.hq % a.qtiles, head0 = c.hq / a.qtiles * a.group + qt * a.gq;
+        const uint32_t kh = a.qtiles > 1 ? c.hq / a.qtiles : c.hq, qt = c.hq - kh * a.qtiles, head0 = kh * a.group + qt * a.gq;
         const uint32_t nq = min(a.gq, a.group - qt * a.gq);
         core.start(a, c.seq, head0, nq, lane, qs);
         for (uint32_t i = 0; i < n; ++i)
@@ -852,7 +898,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
         {
             // CTAs c0 .. c1 hold the item's parts
             const uint64_t item = begin + c.unit - from * kTileUnits;
-            const uint32_t c0 = (uint32_t)(item / per), c1 = (uint32_t)((item + (c.tiles - 1) * (uint64_t)kTileUnits) / per);
+            const uint32_t c0 = (uint32_t)quotient(item, per),
+                           c1 = (uint32_t)quotient(item + (c.tiles - 1) * (uint64_t)kTileUnits, per);
             __syncthreads();
             if (tid == 0)
             {
@@ -950,6 +997,8 @@ extern "C" vkllm_err_t vkllm_b200_paged_attention(const struct vkllm_b200_paged_
     a.cap = (uint32_t)(table_rows(*t) < 0xffffff00ull ? table_rows(*t) : 0xffffff00ull);
     a.q = q, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.lens = lens;
+    a.page_bytes = kv->page_stride * es, a.head_bytes = kv->head_stride * es, a.row_bytes = kv->row_stride * es;
+    a.page_magic = kv->page_rows > 1 ? ~0ull / kv->page_rows + 1 : 0;
     a.group = heads / kv->kv_heads;
     const uint32_t most = kv->dtype == vkllm_dtype_float16 ? 16 : 8; // queries that a CTA takes through one pass
     a.qtiles = (a.group + most - 1) / most;
