@@ -4,20 +4,20 @@
 //   x = x - frequency * (times generated) - (generated ? presence : 0)
 //   x = x + the id's biases;  x = mask bit ? x : -infinity
 //
-// Every logit is read and written once (HBM bounds a large batch, latency a few rows), but the
-// penalties and biases touch at most as many ids as the history and the lists are long. So there are two steps:
+// Every logit is read and written once (HBM bounds a large batch, latency a few rows), but the penalties
+// and biases touch at most as many ids as the history and the lists are long. So there are two steps:
 //   k_logits_copy   streams the rows through, with the mask: out = mask bit ? x : -infinity. In place it writes masked
 //                   logits only, and without a mask it is not launched.
 //   k_logits_touch  one block per row: the touched ids with their counts and bias sums in a hash table in
 //                   shared memory, then x read, ruled, rounded once and written at those ids.
-// The second is the first one's programmatic dependent: it builds its tables while the first streams
-// and waits for it only before it touches the rows. The first's grid is resident at once for that
-// reason. Few rows take one kernel, k_logits_touch<T, true>, whose blocks do both steps for a piece of a row.
-// Counts are integer atomics, and biases are added by one warp in the order of the list: the result does
-// not depend on the order of arrival.
-// 256 rows of 100003 fp16 logits with 1024 to 2048 ids of history, all rules (107 MB): 31.0 us, of which the first kernel
-// alone takes 23 and a plain copy of as much 19. What is left is the second one's scattered reads and writes, 1000
-// ids a row. (All in one kernel of pieces: 62.9 us with counts in arrays over the piece, 44 with hash tables.)
+// The second is the first one's programmatic dependent: it builds its tables while the first streams and
+// waits for it only before it touches the rows. The first's grid is resident at once for that reason. Few
+// rows take one kernel, k_logits_touch<T, true>, whose blocks do both steps for a piece of a row. Counts
+// are integer atomics, and biases are added by one warp in the order of the list: the result does not
+// depend on the order of arrival. 256 rows of 100003 fp16 logits with 1024 to 2048 ids of history, all
+// rules (107 MB): 31.0 us, of which the first kernel alone takes 23 and a plain copy of as much 19. What is
+// left is the second one's scattered reads and writes, 1000 ids a row. (All in one kernel of pieces: 62.9
+// us with counts in arrays over the piece, 44 with hash tables.)
 #include <atomic>
 #include <cmath>
 
@@ -29,9 +29,9 @@ namespace vkb
 namespace
 {
 
-// 16-byte vectors that a thread has in flight, and CTAs per SM: 48 KB of loads, and registers left for a block of the
-// other kernel. (256 rows of 100003 fp16 logits, all rules, when the whole took 31.9 us: 4 vectors x 4 or 5 CTAs 33.8, 33.0; two
-// items in flight a thread 34.1.)
+// 16-byte vectors that a thread has in flight, and CTAs per SM: 48 KB of loads, and registers left for a
+// block of the other kernel. (256 rows of 100003 fp16 logits, all rules, when the whole took 31.9 us: 4
+// vectors x 4 or 5 CTAs 33.8, 33.0; two items in flight a thread 34.1.)
 constexpr uint32_t kCopyThreads = 256, kCopyVecs = 2, kCopyCtas = 6;
 constexpr uint32_t kTouchThreads = 512; // of a row, or half as many where rows share an SM (see launch)
 // Slots of the hash table, 16 bytes each; it takes lists of up to 3/4 as many ids (with repeats), longer ones
@@ -78,10 +78,10 @@ template <> __device__ __forceinline__ uint4 masked<float>(uint4 v, uint32_t bit
     return make_uint4(bits & 1 ? v.x : inf, bits & 2 ? v.y : inf, bits & 4 ? v.z : inf, bits & 8 ? v.w : inf);
 }
 
-// One thread's vectors of a chunk of a row. A row is cut at the 128-byte boundaries of the input, into chunks of
-// equal size: place e of a row is id e - lead, where `lead` elements lie between the boundary at or before the
-// row's start and the row. (Chunks that began at any 16-byte boundary, where warps meet in the middle of lines,
-// copied 51 MB in 24.3 us instead of 21.8.)
+// One thread's vectors of a chunk of a row. A row is cut at the 128-byte boundaries of the input, into
+// chunks of equal size: place e of a row is id e - lead, where `lead` elements lie between the boundary at
+// or before the row's start and the row. (Chunks that began at any 16-byte boundary, where warps meet in
+// the middle of lines, copied 51 MB in 24.3 us instead of 21.8.)
 template <typename T> struct CopyItem
 {
     static constexpr uint32_t E = 16 / sizeof(T), kAll = (1u << E) - 1;
@@ -169,8 +169,8 @@ template <typename T> __global__ void __launch_bounds__(kCopyThreads) k_logits_c
     }
 }
 
-// The touched ids: of a row (one block each), or with PIECE of one chunk of a row, which the block streams through
-// itself before.
+// The touched ids: of a row (one block each), or with PIECE of one chunk of a row, which the block streams
+// through itself before.
 template <typename T, bool PIECE> __global__ void __launch_bounds__(kTouchThreads, 4) k_logits_touch(const RuleArgs a)
 {
     extern __shared__ uint32_t sm[];
@@ -305,9 +305,9 @@ template <typename T, bool PIECE> __global__ void __launch_bounds__(kTouchThread
         if (!waited) // the rows are the first kernel's until it is done
             asm volatile("griddepcontrol.wait;" ::: "memory");
         waited = true;
-        // A row's logits are read back from the output, where the first kernel just put them: they are in L2, while the
-        // input's lines would be fetched from memory once more. A piece's are still there from its own loads (in place
-        // as well: what the mask allows is as it was).
+        // A row's logits are read back from the output, where the first kernel just put them: they are in
+        // L2, while the input's lines would be fetched from memory once more. A piece's are still there
+        // from its own loads (in place as well: what the mask allows is as it was).
         T *y = (T *)a.y + row * a.y_stride;
         const T *in = PIECE ? (const T *)a.x + row * a.x_stride : y;
         for (uint32_t i0 = tid; i0 < n; i0 += 4 * threads)
@@ -367,10 +367,10 @@ template <typename T> vkllm_err_t launch_rules(RuleArgs &a, int sms, int device,
         if (device < 64)
             done[device].store(true, std::memory_order_relaxed);
     }
-    // One kernel while its blocks run at once: each reads the whole history, but nothing waits for a second kernel.
-    // Of 32000 fp16 logits with up to 768 ids of history, 4 / 32 / 64 / 128 rows take 5.7 / 6.9 / 11.0 / 16.8 us in one
-    // kernel and 9.5 / 10.4 / 10.6 / 11.4 in two; of 32000 fp32 ones with up to 5000 ids, where the large table
-    // leaves an SM one block, 16 rows 24.6 and 16.5.
+    // One kernel while its blocks run at once: each reads the whole history, but nothing waits for a second
+    // kernel. Of 32000 fp16 logits with up to 768 ids of history, 4 / 32 / 64 / 128 rows take 5.7 / 6.9 /
+    // 11.0 / 16.8 us in one kernel and 9.5 / 10.4 / 10.6 / 11.4 in two; of 32000 fp32 ones with up to 5000
+    // ids, where the large table leaves an SM one block, 16 rows 24.6 and 16.5.
     if (copy && touch && (uint64_t)a.rows * a.chunks <= (a.slots == kSlotsSmall ? 2 : 1) * (uint64_t)sms)
     {
         k_logits_touch<T, true><<<dim3(a.chunks, a.rows), kCopyThreads, a.slots * 16, s>>>(a);

@@ -62,8 +62,9 @@ inline bool words(const void *p)
     return p && aligned_to(p, 4);
 }
 
-// Refuses arrays that the current device does not own: a launch on them would fault or read across the
-// bus (null pointers are passed over). *sms receives the SM count of the current device. Looking at a pointer takes the host 50 ns.
+// Refuses arrays that the current device does not own: a launch on them would fault or read across the bus
+// (null pointers are passed over). *sms receives the SM count of the current device. Looking at a pointer
+// takes the host 50 ns.
 vkllm_err_t check_device(std::initializer_list<const void *> arrays, int *sms, int *device);
 
 // A table whose shape fits (the pointers' targets are not looked at).

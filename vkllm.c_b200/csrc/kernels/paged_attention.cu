@@ -2,29 +2,32 @@
 //
 //   out = sum_j exp(scale q . k_j - m) v_j / sum_j exp(scale q . k_j - m),  j < len,  m = max_j scale q . k_j
 //
-// Every cached row is read once for all the query heads that share its key head: 2 to 32 flops a byte,
-// so HBM bounds the call, and what matters is that every SM keeps enough loads in flight from the
-// first microsecond to the last.
+// Every cached row is read once for all the query heads that share its key head: 2 to 32 flops a byte, so
+// HBM bounds the call, and what matters is that every SM keeps enough loads in flight from the first
+// microsecond to the last.
 //
 // Work. Lengths are known on the device only, so the kernel divides the work itself. An item is one
-// (sequence, key head, tile of up to 8 or 16 of its queries); its keys are cut into tiles of 4 slices,
-// one slice per warp (16 keys in fp16, 8 in fp32). All tiles of all items form one line, in which an item's end
-// counts too, and every CTA of a grid that fills the GPU takes an equal part of it: a long sequence spreads over all SMs and
-// short ones share a CTA. A CTA that holds only a part of an item leaves (m, l, O) in the workspace and counts
-// itself at the item; the last one to arrive joins the parts in the order of the line, so the result
-// does not depend on who was last. (Handing the last quarter of the line out in small chunks off a ticket
-// counter was slower: 98 instead of 78 us for 64 sequences of 128 to 640 keys, since every chunk refills the rings.)
+// (sequence, key head, tile of up to 8 or 16 of its queries); its keys are cut into tiles of 4 slices, one
+// slice per warp (16 keys in fp16, 8 in fp32). All tiles of all items form one line, in which an item's end
+// counts too, and every CTA of a grid that fills the GPU takes an equal part of it: a long sequence spreads
+// over all SMs and short ones share a CTA. A CTA that holds only a part of an item leaves (m, l, O) in the
+// workspace and counts itself at the item; the last one to arrive joins the parts in the order of the line,
+// so the result does not depend on who was last. (Handing the last quarter of the line out in small chunks
+// off a ticket counter was slower: 98 instead of 78 us for 64 sequences of 128 to 640 keys, since every
+// chunk refills the rings.)
 //
 // Loads. Each warp streams its own slices through a private ring of cp.async stages, also across the
-// borders of items: no barrier of the CTA stands between a load and its use. Page ids are read one tile ahead of
-// the rows that they lead to. Rows past the end, and rows of bad pages, are filled with zeros without being read and masked out of the scores.
+// borders of items: no barrier of the CTA stands between a load and its use. Page ids are read one tile
+// ahead of the rows that they lead to. Rows past the end, and rows of bad pages, are filled with zeros
+// without being read and masked out of the scores.
 //
 // fp16: S^T = K Q^T on the tensor cores (mma.sync m16n8k16: 16 keys x 8 queries), so that the 8 columns
-// take up to 8 queries that share the keys and each lane keeps the statistics of two of them; then O^T += V^T P with
-// P^T moved into operand order by movmatrix. The weights are kept as the sum of two fp16 parts, scaled by
-// 2^15: one part alone would double the error of the rounded output, and unscaled ones would lose their bits
-// below fp16's range where one key outweighs very many small ones (the tensor cores have the time: they idle behind the loads).
-// fp32: plain FMAs; 4 lanes share a key's dot product, and every lane owns head_dim / 32 of the output.
+// take up to 8 queries that share the keys and each lane keeps the statistics of two of them; then O^T +=
+// V^T P with P^T moved into operand order by movmatrix. The weights are kept as the sum of two fp16 parts,
+// scaled by 2^15: one part alone would double the error of the rounded output, and unscaled ones would lose
+// their bits below fp16's range where one key outweighs very many small ones (the tensor cores have the
+// time: they idle behind the loads). fp32: plain FMAs; 4 lanes share a key's dot product, and every lane
+// owns head_dim / 32 of the output.
 #include <atomic>
 #include <type_traits>
 
@@ -69,8 +72,8 @@ struct PagedAttArgs
 
 constexpr uint32_t kRound = 4; // queries that the join buffers take at a time
 
-// KD: dimensions that are computed, head_dim rounded up; HP: those that a row in shared memory has room for, a power of
-// two, so that its 16-byte pieces can be swizzled.
+// KD: dimensions that are computed, head_dim rounded up; HP: those that a row in shared memory has room
+// for, a power of two, so that its 16-byte pieces can be swizzled.
 template <typename T, int KD> struct Shape
 {
     static constexpr int HP = KD <= 64 ? 64 : KD <= 128 ? 128 : 256;
@@ -166,8 +169,8 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b)
     return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
 }
 
-// A place in the line of tiles: tile `tile` of `tiles` of item (seq, hq), hq = key head * qtiles + query tile, `unit`
-// units behind the start of the CTA's part.
+// A place in the line of tiles: tile `tile` of `tiles` of item (seq, hq), hq = key head * qtiles + query
+// tile, `unit` units behind the start of the CTA's part.
 struct Cursor
 {
     uint32_t seq, hq, tile, tiles, len, unit;
@@ -198,8 +201,9 @@ struct Cursor
     }
 };
 
-// The stream of one warp's slices: page ids one tile ahead, rows kStages - 1 tiles ahead. A warp issues a few hundred
-// instructions for a tile, with no other warp to hide their latency behind in a short call, so what can be worked out before is.
+// The stream of one warp's slices: page ids one tile ahead, rows kStages - 1 tiles ahead. A warp issues a
+// few hundred instructions for a tile, with no other warp to hide their latency behind in a short call, so
+// what can be worked out before is.
 template <typename T, int KD, bool EXACT> struct Loader
 {
     using S = Shape<T, KD>;
@@ -430,7 +434,8 @@ template <int KD, int NQ, bool EXACT> struct HalfCore
         }
     }
 
-    // Queries kRound r .. of the item, those below nq, into the warp's join buffer: os [kRound][kPitch], ml [kRound][2].
+    // Queries kRound r .. of the item, those below nq, into the warp's join buffer: os [kRound][kPitch], ml
+    // [kRound][2].
     __device__ __forceinline__ void deposit(int r, uint32_t nq, float *os, float *ml, uint32_t lane)
     {
 #pragma unroll
@@ -624,7 +629,8 @@ __device__ __forceinline__ void add_scaled(float4 &o, float f, const float4 &v)
     o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
 }
 
-// A join buffer, joined over the warps: queries q0 .. q0 + n - 1 of the item (at most kRound), to the output or to a part.
+// A join buffer, joined over the warps: queries q0 .. q0 + n - 1 of the item (at most kRound), to the
+// output or to a part.
 template <typename T, int KD>
 __device__ __forceinline__ void join_warps(const PagedAttArgs &a, const float *os, const float *ml, uint32_t n,
                                            uint32_t q0, uint32_t seq, uint32_t head0, float *part)
@@ -658,16 +664,17 @@ __device__ __forceinline__ void join_warps(const PagedAttArgs &a, const float *o
     }
 }
 
-// The part of CTA c of an item that begins in CTA c0: a CTA's second place is for the item that begins in it and goes on.
+// The part of CTA c of an item that begins in CTA c0: a CTA's second place is for the item that begins in
+// it and goes on.
 __device__ __forceinline__ float *part_of(const PagedAttArgs &a, uint32_t c, bool begins)
 {
     return a.parts + (2 * (uint64_t)c + begins) * a.part_stride;
 }
 
-// An item joined over its parts in CTAs c0 .. c1, in their order, to the output. What it costs is the latency of its loads, at
-// the end of a CTA's work: so every thread takes 4 elements of a query with the statistics of their parts on its
-// own, 16 parts in flight, and where the item has too few elements to fill the CTA, and parts enough, groups of
-// threads take every `groups`-th part and meet in shared memory.
+// An item joined over its parts in CTAs c0 .. c1, in their order, to the output. What it costs is the
+// latency of its loads, at the end of a CTA's work: so every thread takes 4 elements of a query with the
+// statistics of their parts on its own, 16 parts in flight, and where the item has too few elements to fill
+// the CTA, and parts enough, groups of threads take every `groups`-th part and meet in shared memory.
 template <typename T, int KD>
 __device__ __noinline__ void join_parts(const PagedAttArgs &a, uint32_t c0, uint32_t c1, float *sm, uint32_t nq,
                                         uint32_t seq, uint32_t head0)

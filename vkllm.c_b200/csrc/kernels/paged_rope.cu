@@ -2,19 +2,20 @@
 //
 //   (a, b) -> (a cos t - b sin t, a sin t + b cos t),  t = position * base^(-2w / hd),  pairs (2w, 2w + 1)
 //
-// on q (to q_out) and k (to the slot's key row); v is copied to the slot's value row. The pairs are
-// those of VKLLM_OP_ROPE. Every element is read and written once, so a long call is bound by HBM and a
-// short one by latency.
+// on q (to q_out) and k (to the slot's key row); v is copied to the slot's value row. The pairs are those
+// of VKLLM_OP_ROPE. Every element is read and written once, so a long call is bound by HBM and a short one
+// by latency.
 //
 // Angles: fp32 loses the angle of far positions (at position 200000 the rounding of position * frequency
-// alone is 8e-3 radians). The frequency is kept as a fraction of a turn in 64-bit fixed point,
-// f = base^(-2w / hd) / (2 pi) < 2^-2, so position * f modulo 2^64 is the exact fraction of the last turn for the
-// rounded f: an error of at most position * 2^-64 turns, and no range reduction. sincospif takes it
+// alone is 8e-3 radians). The frequency is kept as a fraction of a turn in 64-bit fixed point, f =
+// base^(-2w / hd) / (2 pi) < 2^-2, so position * f modulo 2^64 is the exact fraction of the last turn for
+// the rounded f: an error of at most position * 2^-64 turns, and no range reduction. sincospif takes it
 // from there in fp32.
 //
-// A block works out a token's sines and cosines once, into shared memory; each thread owns one 16-byte piece of a
-// head (4 or 2 pairs), keeps those of its pairs, and walks over its share of the token's heads, 4 loads in flight.
-// 2048 tokens of 40 + 80 heads of 128 (126 MB, fp16): 24.6 us, 5.1 TB/s, where a plain copy of 102 MB reaches 5.5.
+// A block works out a token's sines and cosines once, into shared memory; each thread owns one 16-byte
+// piece of a head (4 or 2 pairs), keeps those of its pairs, and walks over its share of the token's heads,
+// 4 loads in flight. 2048 tokens of 40 + 80 heads of 128 (126 MB, fp16): 24.6 us, 5.1 TB/s, where a plain
+// copy of 102 MB reaches 5.5.
 #include <cmath>
 
 #include "paged.cuh"
@@ -76,8 +77,8 @@ template <> struct Piece<float>
     }
 };
 
-// Block: a multiple of the pieces of a head; grid.x: tokens, grid.y: shares of the token's rows (q heads, then key heads,
-// then value heads).
+// Block: a multiple of the pieces of a head; grid.x: tokens, grid.y: shares of the token's rows (q heads,
+// then key heads, then value heads).
 template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_rope_write(const RopeArgs a)
 {
     constexpr int P = Piece<T>::kPairs, E = 2 * P;
@@ -183,8 +184,9 @@ extern "C" vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged
     for (uint32_t w = 0; w < hd / 2; ++w, f *= ratio)
         a.turns[w] = (uint64_t)f;
     const uint32_t pieces = hd * es / 16, threads = kRopeThreads / pieces * pieces, lanes = threads / pieces;
-    // Blocks of a token: so many that a thread has one batch of rows in flight (2048 tokens of 120 heads: 2 blocks
-    // a token 24.6 us, one 25.9), and of few tokens more, until the call reaches about two blocks an SM.
+    // Blocks of a token: so many that a thread has one batch of rows in flight (2048 tokens of 120 heads: 2
+    // blocks a token 24.6 us, one 25.9), and of few tokens more, until the call reaches about two blocks an
+    // SM.
     const uint32_t passes = (heads + 2 * kv->kv_heads + lanes - 1) / lanes;
     uint32_t shares = (passes + kRopeAhead - 1) / kRopeAhead;
     while (shares < passes && (uint64_t)n_tokens * shares < 2u * (uint32_t)sms)

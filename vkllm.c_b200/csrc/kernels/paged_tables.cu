@@ -10,12 +10,11 @@
 // The floor is the words in and out (8 bytes a token and 20 a sequence), microseconds at most: the calls
 // are bound by the latency of one launch and of a few dependent loads.
 //
-// One thread-block cluster does a call (but for the slots of many tokens, which a second kernel spreads over the GPU).
-// Every CTA sums all sequences itself (they are few; a scan split over CTAs
-// would need an exchange more) into shared memory, then takes its share of the tokens, pages and
-// sequences, found by binary search in the sums, so one long prompt among many short ones spreads
-// evenly. The cluster barrier between the last read and the first write is what makes all-or-nothing
-// and new_lens == lens possible.
+// One thread-block cluster does a call (but for the slots of many tokens, which a second kernel spreads
+// over the GPU). Every CTA sums all sequences itself (they are few; a scan split over CTAs would need an
+// exchange more) into shared memory, then takes its share of the tokens, pages and sequences, found by
+// binary search in the sums, so one long prompt among many short ones spreads evenly. The cluster barrier
+// between the last read and the first write is what makes all-or-nothing and new_lens == lens possible.
 #include <atomic>
 #include <cooperative_groups.h>
 #include <new>
@@ -56,8 +55,9 @@ namespace
 constexpr uint32_t kMaxSeqs = 16384; // three words a sequence in shared memory
 constexpr uint32_t kTabThreads = 512;
 constexpr uint32_t kMaxCluster = 8;
-// Most tokens whose slots the cluster writes itself. More go to a second kernel over the whole GPU: a release and an
-// append of 131072 tokens in 512 sequences took 23.9 us with one cluster for all, and take 13.5 this way.
+// Most tokens whose slots the cluster writes itself. More go to a second kernel over the whole GPU: a
+// release and an append of 131072 tokens in 512 sequences took 23.9 us with one cluster for all, and take
+// 13.5 this way.
 constexpr uint32_t kTokensHere = kMaxCluster * kTabThreads;
 constexpr uint32_t kSlotThreads = 256;
 
@@ -225,8 +225,8 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_append(const AppendArgs a
     }
 }
 
-// Slots and positions of many tokens, from what k_paged_append left: runs of four per thread, which mostly share
-// their sequence, its search and its page.
+// Slots and positions of many tokens, from what k_paged_append left: runs of four per thread, which mostly
+// share their sequence, its search and its page.
 __global__ void __launch_bounds__(kSlotThreads) k_paged_slots(const AppendArgs a)
 {
     extern __shared__ uint32_t starts[];
