@@ -58,7 +58,7 @@ struct PagedAttArgs
     void *out;
     uint64_t q_stride, out_stride;
     uint64_t page_bytes, head_bytes, row_bytes; // strides of the pools
-    uint64_t page_magic; // ceil(2^64 / page_rows): its product with a key's number has the page's column above bit 64; 0: one row
+    uint64_t page_magic; // ceil(2^64 / page_rows), to divide a key's number by page_rows; 0: page_rows is 1
     const uint32_t *lens;
     uint32_t group;  // queries that share a key head
     uint32_t qtiles; // tiles of these queries
@@ -70,23 +70,34 @@ struct PagedAttArgs
     uint32_t part_stride;
 };
 
-constexpr uint32_t kRound = 4; // queries that the join buffers take at a time
-
-// KD: dimensions that are computed, head_dim rounded up; HP: those that a row in shared memory has room
-// for, a power of two, so that its 16-byte pieces can be swizzled.
+// Shared memory for a head size. KD: dimensions that are computed, head_dim rounded up. Rows must not meet in the same banks
+// where 8 of them are read at once: a power of two of 16-byte pieces is swizzled, other rows get a piece more.
 template <typename T, int KD> struct Shape
 {
-    static constexpr int HP = KD <= 64 ? 64 : KD <= 128 ? 128 : 256;
+    static constexpr bool kPow2 = (KD & (KD - 1)) == 0;
     static constexpr uint32_t kKeys = sizeof(T) == 2 ? 16 : 8;                  // keys of a slice
-    static constexpr uint32_t kRow = HP * sizeof(T);                            // bytes of a row in shared memory
+    static constexpr uint32_t kRow = KD * sizeof(T) + (kPow2 ? 0 : 16);         // bytes of a row
     static constexpr uint32_t kStage = 2 * kKeys * kRow;                        // K and V of a slice
     static constexpr uint32_t kQBytes = sizeof(T) == 4 ? 8 * KD * 4 : 0;        // the queries (fp32 only)
-    static constexpr uint32_t kStages = HP == 64 ? (sizeof(T) == 4 ? 3 : 4) : sizeof(T) == 4 ? 2 : 3;
-    static constexpr uint32_t kPitch = KD + 4;                                  // floats of a row of the join buffer
+    // Stages of a warp's ring, CTAs of an SM and queries that a join buffer takes. Small heads need more warps for
+    // the same bytes: 8 x 16 heads of 64 with 4096 keys take 31.7 us with 3 CTAs of 4 stages, 35.9 with 2 of 6; 28
+    // heads of 80 over 4 take 72 with 3 of 2 and 80 with 2 of 3. Of 128, 3 CTAs of 2 stages (kRound 2) are better
+    // where items are short (200 sequences of up to 120 keys: 48 instead of 57 us) and worse where they are long or
+    // 16 queries share a head (65 instead of 59), so it stays at 2 of 3.
+    static constexpr uint32_t kStages = KD <= 64 ? (sizeof(T) == 4 ? 3 : 4) : sizeof(T) == 4 || KD == 96 ? 2 : 3;
+    static constexpr uint32_t kCtas = KD > 128 ? 1 : KD <= 96 ? 3 : 2;
+    static constexpr uint32_t kRound = 4;
+    static constexpr uint32_t kPitch = KD + 4;                                  // floats of a row of a join buffer
     static constexpr uint32_t kRing = kWarps * kStages * kStage;
-    static constexpr uint32_t kJoin = kWarps * kRound * (kPitch + 2);           // floats of a join buffer: O, then m and l
+    static constexpr uint32_t kJoin = kWarps * kRound * (kPitch + 2); // floats of a join buffer: O, then m and l
     static constexpr uint32_t kSmem = kRing + kQBytes + 2 * kJoin * 4 + kWarps * kStages * 4;
-    static constexpr uint32_t kCtas = HP == 256 ? 1 : HP == 64 ? 3 : 2; // per SM
+    static_assert(kSmem <= 227 * 1024 && kCtas * (kSmem + 1200) <= 228 * 1024, "shared memory of an SM");
+
+    // Byte of 16-byte piece p of row r.
+    static __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t p)
+    {
+        return r * kRow + (kPow2 ? p ^ (r & 7) : p) * 16;
+    }
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes)
@@ -208,7 +219,8 @@ template <typename T, int KD, bool EXACT> struct Loader
 {
     using S = Shape<T, KD>;
     static constexpr uint32_t kPieces = KD * sizeof(T) / 16;
-    static constexpr bool kFixed = EXACT && 32 % kPieces == 0; // a lane copies the same piece of every row that it copies
+    // a lane copies the same piece of every row that it copies
+    static constexpr bool kFixed = EXACT && S::kPow2 && kPieces <= 32;
     Cursor c;
     uint32_t end;       // units of the CTA's part
     uint32_t page, row; // of key `lane % kKeys` of the slice at c, and its row in the page
@@ -302,7 +314,7 @@ template <typename T, int KD, bool EXACT> struct Loader
                         const uint32_t bytes = (mask >> r) & 1u ? 16u : 0u;
                         if (EXACT || r0 < S::kKeys)
                         {
-                            const uint32_t dst = base + r * S::kRow + ((p ^ (r & 7)) * 16);
+                            const uint32_t dst = base + S::at(r, p);
                             cp_async16(dst, k + off, bytes);
                             cp_async16(dst + S::kKeys * S::kRow, v + off, bytes);
                         }
@@ -373,7 +385,7 @@ template <int KD, int NQ, bool EXACT> struct HalfCore
         for (int k = 0; k < kK; ++k)
         {
             uint32_t f[4];
-            ldsm4(f, base + kr * S::kRow + (((2 * k + (lane >> 4)) ^ (kr & 7)) * 16));
+            ldsm4(f, base + S::at(kr, 2 * k + (lane >> 4)));
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
                 mma16816(s[n][k & 1], f, qf[n][k][0], qf[n][k][1]);
@@ -419,12 +431,12 @@ template <int KD, int NQ, bool EXACT> struct HalfCore
                 lo[n][b] = transpose8x8(pack2(x[2 * b] - hf.x, x[2 * b + 1] - hf.y));
             }
         }
-        const uint32_t vr = (lane & 7) + ((lane >> 4) & 1) * 8, vbase = base + S::kKeys * S::kRow + vr * S::kRow;
+        const uint32_t vr = (lane & 7) + ((lane >> 4) & 1) * 8, vbase = base + S::kKeys * S::kRow;
 #pragma unroll
         for (int k = 0; k < kK; ++k)
         {
             uint32_t f[4];
-            ldsm4_t(f, vbase + (((2 * k + ((lane >> 3) & 1)) ^ (vr & 7)) * 16));
+            ldsm4_t(f, vbase + S::at(vr, 2 * k + ((lane >> 3) & 1)));
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
             {
@@ -434,13 +446,13 @@ template <int KD, int NQ, bool EXACT> struct HalfCore
         }
     }
 
-    // Queries kRound r .. of the item, those below nq, into the warp's join buffer: os [kRound][kPitch], ml
-    // [kRound][2].
+    // Queries kRound r .. of the item, those below nq, into the warp's join buffer: os [kRound][kPitch], ml [kRound][2].
     __device__ __forceinline__ void deposit(int r, uint32_t nq, float *os, float *ml, uint32_t lane)
     {
+        constexpr uint32_t kPairs = S::kRound / 2, kPer = 8 / S::kRound; // pairs of queries of a round; rounds of 8
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
-            if (n == r / 2)
+            if (n == r / (int)kPer)
             {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -449,9 +461,9 @@ template <int KD, int NQ, bool EXACT> struct HalfCore
                     t += __shfl_xor_sync(0xffffffffu, t, 4);
                     t += __shfl_xor_sync(0xffffffffu, t, 8);
                     t += __shfl_xor_sync(0xffffffffu, t, 16);
-                    // this lane's query is 8 n + 2 (lane & 3) + i
-                    const uint32_t q = (lane & 1) * 2 + i;
-                    if ((lane >> 1 & 1u) != (uint32_t)(r & 1) || r * kRound + q >= nq)
+                    // this lane's query is 8 n + 2 pair + i
+                    const uint32_t pair = lane & 3, q = pair % kPairs * 2 + i;
+                    if (pair / kPairs != r % kPer || r * S::kRound + q >= nq)
                         continue;
                     if (lane < 4)
                         ml[q * 2] = m[n][i], ml[q * 2 + 1] = t;
@@ -473,9 +485,10 @@ template <int KD, int NQ, bool EXACT> struct FloatCore
     using T = float;
     using S = Shape<T, KD>;
     static constexpr int kQueries = NQ;
-    static constexpr int kP = S::HP / 4;                    // pieces that a row has room for
-    static constexpr int kOwn = kP > 32 ? kP / 32 : 1;      // pieces that a lane owns
-    static constexpr int kHalves = kP < 32 ? 32 / kP : 1;   // lane groups that share the keys (KD = 64: 2)
+    static constexpr int kP = KD / 4;                       // pieces of a row
+    static constexpr int kRowP = S::kRow / 16;              // and from row to row
+    static constexpr int kOwn = (kP + 31) / 32;             // pieces that a lane owns
+    static constexpr int kHalves = kP == 16 ? 2 : 1;      // lane groups that share the keys (KD = 64: 2)
     float4 o[NQ][kOwn];
     float m[NQ], l[NQ];
 
@@ -504,7 +517,7 @@ template <int KD, int NQ, bool EXACT> struct FloatCore
         extern __shared__ __align__(128) unsigned char sm[];
         const uint32_t off = base - (uint32_t)__cvta_generic_to_shared(sm);
         const float4 *K = reinterpret_cast<const float4 *>(sm + off);
-        const float4 *V = K + S::kKeys * kP;
+        const float4 *V = K + S::kKeys * kRowP;
         const uint32_t key = lane & 7, part = lane >> 3;
         // every query's dot product in two chains (even and odd elements), all queries side by side
         float2 d[NQ];
@@ -514,7 +527,7 @@ template <int KD, int NQ, bool EXACT> struct FloatCore
 #pragma unroll
         for (int j = 0; j < KD / 16; ++j)
         {
-            const float4 k = K[key * kP + ((4 * j + part) ^ key)];
+            const float4 k = K[S::at(key, 4 * j + part) / 16];
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
             {
@@ -559,7 +572,7 @@ template <int KD, int NQ, bool EXACT> struct FloatCore
 #pragma unroll
                 for (int k = 0; k < kOwn; ++k)
                     o[i][k].x *= f[i], o[i][k].y *= f[i], o[i][k].z *= f[i], o[i][k].w *= f[i];
-        const uint32_t own = lane % kP, first = kHalves > 1 ? lane / kP : 0;
+        const uint32_t first = kHalves > 1 ? lane / kP : 0;
 #pragma unroll
         for (uint32_t j = 0; j < S::kKeys / kHalves; ++j)
         {
@@ -567,7 +580,7 @@ template <int KD, int NQ, bool EXACT> struct FloatCore
             float4 v[kOwn];
 #pragma unroll
             for (int k = 0; k < kOwn; ++k)
-                v[k] = V[r * kP + ((own + 32 * k) ^ (r & 7))];
+                v[k] = V[S::at(r, (lane + 32 * k) % kP) / 16]; // (a lane without a piece takes another's)
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
             {
@@ -588,9 +601,9 @@ template <int KD, int NQ, bool EXACT> struct FloatCore
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
         {
-            if (i / kRound != r || i >= nq)
+            if (i / (int)S::kRound != r || i >= nq)
                 continue;
-            const uint32_t q = i % kRound;
+            const uint32_t q = i % S::kRound;
             float t = l[i];
             t += __shfl_xor_sync(0xffffffffu, t, 1);
             t += __shfl_xor_sync(0xffffffffu, t, 2);
@@ -606,8 +619,8 @@ template <int KD, int NQ, bool EXACT> struct FloatCore
                     v.x += __shfl_xor_sync(0xffffffffu, v.x, 16), v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
                     v.z += __shfl_xor_sync(0xffffffffu, v.z, 16), v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
                 }
-                if (lane % kP + 32 * k < KD / 4 && (kHalves == 1 || lane < kP))
-                    *reinterpret_cast<float4 *>(os + q * S::kPitch + 4 * (lane % kP + 32 * k)) = v;
+                if (lane + 32 * k < kP)
+                    *reinterpret_cast<float4 *>(os + q * S::kPitch + 4 * (lane + 32 * k)) = v;
             }
         }
     }
@@ -629,7 +642,7 @@ __device__ __forceinline__ void add_scaled(float4 &o, float f, const float4 &v)
     o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
 }
 
-// A join buffer, joined over the warps: queries q0 .. q0 + n - 1 of the item (at most kRound), to the
+// A join buffer, joined over the warps: queries q0 .. q0 + n - 1 of the item (at most S::kRound), to the
 // output or to a part.
 template <typename T, int KD>
 __device__ __forceinline__ void join_warps(const PagedAttArgs &a, const float *os, const float *ml, uint32_t n,
@@ -642,16 +655,16 @@ __device__ __forceinline__ void join_warps(const PagedAttArgs &a, const float *o
         float mx = -INFINITY;
 #pragma unroll
         for (uint32_t w = 0; w < kWarps; ++w)
-            mx = fmaxf(mx, ml[(w * kRound + q) * 2]);
+            mx = fmaxf(mx, ml[(w * S::kRound + q) * 2]);
         const float b = finite_base(mx);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         float l = 0.f;
 #pragma unroll
         for (uint32_t w = 0; w < kWarps; ++w)
         {
-            const float f = pow2(ml[(w * kRound + q) * 2] - b);
-            l = fmaf(f, ml[(w * kRound + q) * 2 + 1], l);
-            add_scaled(o, f, *reinterpret_cast<const float4 *>(os + (w * kRound + q) * S::kPitch + d));
+            const float f = pow2(ml[(w * S::kRound + q) * 2] - b);
+            l = fmaf(f, ml[(w * S::kRound + q) * 2 + 1], l);
+            add_scaled(o, f, *reinterpret_cast<const float4 *>(os + (w * S::kRound + q) * S::kPitch + d));
         }
         if (part)
         {
@@ -755,10 +768,11 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
     using S = Shape<T, KD>;
     using Core = Kind<KD, NQ, EXACT>;
     constexpr uint32_t kTile = kWarps * S::kKeys;
-    constexpr int kRounds = (Core::kQueries + kRound - 1) / kRound;
+    constexpr int kRounds = (Core::kQueries + S::kRound - 1) / S::kRound;
     extern __shared__ __align__(128) unsigned char sm[];
     float *qs = reinterpret_cast<float *>(sm + S::kRing);
-    float *join = reinterpret_cast<float *>(sm + S::kRing + S::kQBytes); // two buffers: one is joined while the other fills
+    // two join buffers: one is joined while the other fills
+    float *join = reinterpret_cast<float *>(sm + S::kRing + S::kQBytes);
     uint32_t *valid = reinterpret_cast<uint32_t *>(join + 2 * S::kJoin); // [kWarps][kStages]
     __shared__ uint64_t sums[kWarps];
     __shared__ Cursor first;
@@ -772,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
         for (uint32_t i = tid; i < kWarps * S::kStages * S::kKeys * gap; i += kThreads)
         {
             const uint32_t row = i / gap, r = row % S::kKeys, p = have + i % gap;
-            *reinterpret_cast<uint4 *>(sm + row / S::kKeys * S::kStage + r * S::kRow + (p ^ (r & 7)) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(sm + row / S::kKeys * S::kStage + S::at(r, p)) = make_uint4(0, 0, 0, 0);
         }
     }
 
@@ -845,7 +859,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
         }
         units = max(units, 1u);
         c.hq = (uint32_t)quotient(begin - at, units);
-        const uint32_t x = (uint32_t)(begin - at - (uint64_t)c.hq * units); // a tile is the CTA's in whose part its first unit lies
+        // a tile is the CTA's in whose part its first unit lies
+        const uint32_t x = (uint32_t)(begin - at - (uint64_t)c.hq * units);
         c.tile = (x + kTileUnits - 1) / kTileUnits;
         c.unit = c.tile * kTileUnits - x;
         if (c.tile >= c.tiles)
@@ -874,7 +889,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
     {
         // one item, or this CTA's part of it
         const uint32_t from = c.tile, n = min(c.tiles - from, (end - c.unit + kTileUnits - 1) / kTileUnits);
-        const uint32_t kh = a.qtiles > 1 ? c.hq / a.qtiles : c.hq, qt = c.hq - kh * a.qtiles, head0 = kh * a.group + qt * a.gq;
+        const uint32_t kh = a.qtiles > 1 ? c.hq / a.qtiles : c.hq, qt = c.hq - kh * a.qtiles;
+        const uint32_t head0 = kh * a.group + qt * a.gq;
         const uint32_t nq = min(a.gq, a.group - qt * a.gq);
         core.start(a, c.seq, head0, nq, lane, qs);
         for (uint32_t i = 0; i < n; ++i)
@@ -892,13 +908,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, KD>::kCtas) k_paged_attenti
 #pragma unroll
         for (int r = 0; r < kRounds; ++r)
         {
-            if (r * kRound >= nq)
+            if (r * S::kRound >= nq)
                 break;
             // the barrier also says that every warp is done with the other buffer
-            float *os = join + buffer * S::kJoin, *ml = os + kWarps * kRound * S::kPitch;
-            core.deposit(r, nq, os + warp * kRound * S::kPitch, ml + warp * kRound * 2, lane);
+            float *os = join + buffer * S::kJoin, *ml = os + kWarps * S::kRound * S::kPitch;
+            core.deposit(r, nq, os + warp * S::kRound * S::kPitch, ml + warp * S::kRound * 2, lane);
             __syncthreads();
-            join_warps<T, KD>(a, os, ml, min(nq - r * kRound, kRound), r * kRound, c.seq, head0, part);
+            join_warps<T, KD>(a, os, ml, min(nq - r * S::kRound, S::kRound), r * S::kRound, c.seq, head0, part);
             buffer ^= 1;
         }
         if (!whole)
