@@ -161,6 +161,47 @@ def test_append(vk, torch, n, page_rows, cols, hi, max_tokens, in_place):
     b.same(got, want)
 
 
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_append_of_many_tokens_to_any_alignment(vk, torch, shift):
+    """The slot map's outputs on no 16-byte boundary, both of them or one."""
+    b = Book(vk, torch, [30, 0, 9], 1000, 7, spare=1500, seed=6)
+    new, most = [3000, 1, 2500], 5502 + shift
+    slots, pos = (torch.full((most + 8,), 0x55, dtype=torch.int32, device="cuda") for _ in range(2))
+    starts = torch.zeros(4, dtype=torch.int32, device="cuda")
+    ps, pp = slots.data_ptr() + 4 * shift, pos.data_ptr() + 4 * (shift if shift != 2 else 0)
+    err = vk.lib().vkllm_b200_paged_append(C.byref(b.c_table()), b.d_lens.data_ptr(), i32(torch, new).data_ptr(),
+                                           b.d_count.data_ptr(), b.d_lens.data_ptr(), b.d_count.data_ptr(),
+                                           starts.data_ptr(), ps, pp, most, b.status.data_ptr(), stream(torch))
+    assert err == vk.OK
+    torch.cuda.synchronize()
+    want, st = b.want_append(new, most)
+    at = shift if shift != 2 else 0
+    assert st == 0 and int(b.status) == 0
+    assert np.array_equal(u32(slots)[shift:shift + most], want[3]) and np.array_equal(u32(pos)[at:at + most], want[4])
+    assert (u32(slots)[shift + most:] == 0x55).all() and (u32(slots)[:shift] == 0x55).all()
+    assert (u32(pos)[at + most:] == 0x55).all()
+
+
+def test_append_with_slots_past_31_bits(vk, torch):
+    """Pages of 2^24 rows: lengths, positions and slots beyond 2^31, and a capacity beyond 2^32."""
+    R = 1 << 24
+    b = Book(vk, torch, [100 * R + R - 3, 30 * R, 0, 77 * R + 5], 400, R, spare=20, seed=8)
+    new = [6, 2, 1, 4]
+    got = b.append(new, 15)
+    slots = []
+    for s, (l, m) in enumerate(zip([100 * R + R - 3, 30 * R, 0, 77 * R + 5], new)):
+        for p in range(l, l + m):
+            if p % R == 0:
+                b.count -= 1
+                b.table[s, p // R] = b.free[b.count]
+            slots.append(int(b.table[s, p // R]) * R + p % R)
+    b.lens = (b.lens + np.asarray(new, dtype=np.uint32)).astype(np.uint32)
+    assert int(b.status) == 0 and max(slots) >= 1 << 31
+    want = (b.lens, b.count, [0, 6, 8, 9, 13], slots + [0xffffffff] * 2,
+            [p for l, m in zip([100 * R + R - 3, 30 * R, 0, 77 * R + 5], new) for p in range(l, l + m)] + [0, 0])
+    b.same(got, want)
+
+
 def test_append_exactly_what_is_free_and_nothing(vk, torch):
     b = Book(vk, torch, [4, 0, 3], 4, 4, spare=3)
     b.same(b.append([1, 4, 5], 10), b.want_append([1, 4, 5], 10)[0])  # 1 + 1 + 1 pages: the list is empty now
