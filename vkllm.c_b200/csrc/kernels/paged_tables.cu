@@ -376,7 +376,7 @@ vkllm_err_t launch_cluster(void (*kernel)(const Args), const Args &args, uint32_
     at[0].val.clusterDim.x = ctas;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = ctas > 1 ? 1 : 0;
     VKB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
     return VKLLM_ERR_OK;
 }
