@@ -15,7 +15,7 @@
 // rows take one kernel, k_logits_touch<T, true>, whose blocks do both steps for a piece of a row. Counts
 // are integer atomics, and biases are added by one warp in the order of the list: the result does not
 // depend on the order of arrival. 256 rows of 100003 fp16 logits with 1024 to 2048 ids of history, all
-// rules (107 MB): 31.0 us, of which the first kernel alone takes 23 and a plain copy of as much 19. What is
+// rules (107 MB): 30.9 us, of which the first kernel alone takes 23 and a plain copy of as much 19. What is
 // left is the second one's scattered reads and writes, 1000 ids a row. (All in one kernel of pieces: 62.9
 // us with counts in arrays over the piece, 44 with hash tables.)
 #include <atomic>
@@ -29,14 +29,14 @@ namespace vkb
 namespace
 {
 
-// 16-byte vectors that a thread has in flight, and CTAs per SM: 48 KB of loads, and registers left for a
-// block of the other kernel. (256 rows of 100003 fp16 logits, all rules, when the whole took 31.9 us: 4
-// vectors x 4 or 5 CTAs 33.8, 33.0; two items in flight a thread 34.1.)
-constexpr uint32_t kCopyThreads = 256, kCopyVecs = 2, kCopyCtas = 6;
+// 16-byte vectors that a thread has in flight, and CTAs per SM: 40 KB of loads, and registers left for two
+// blocks of the other kernel. (256 rows of 100003 fp16 logits, all rules: 30.9 us; with 6 CTAs, which leave
+// it fewer registers, 31.1 to 34.4, with 4 31.7; 4 vectors x 4 CTAs 33.8; two items in flight a thread 34.1.)
+constexpr uint32_t kCopyThreads = 256, kCopyVecs = 2, kCopyCtas = 5;
 constexpr uint32_t kTouchThreads = 512; // of a row, or half as many where rows share an SM (see launch)
 // Slots of the hash table, 16 bytes each; it takes lists of up to 3/4 as many ids (with repeats), longer ones
 // go over ranges of the vocabulary instead. The small table lets more rows share an SM.
-constexpr uint32_t kSlotsSmall = 4096, kSlotsLarge = 8192;
+constexpr uint32_t kSlotsSmall = 4096, kSlotsLarge = 8192, kLeastSlots = 512;
 constexpr uint32_t kNoId = 0xffffffffu; // not an id: vocab < 2^31
 constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u; // in the prompt; in the biases; the bits below: times generated
 
@@ -171,9 +171,9 @@ template <typename T> __global__ void __launch_bounds__(kCopyThreads) k_logits_c
 
 // The touched ids: of a row (one block each), or with PIECE of one chunk of a row, which the block streams
 // through itself before.
-template <typename T, bool PIECE> __global__ void __launch_bounds__(kTouchThreads, 4) k_logits_touch(const RuleArgs a)
+template <typename T, bool PIECE> __global__ void __launch_bounds__(PIECE ? kCopyThreads : kTouchThreads, PIECE ? 4 : 3) k_logits_touch(const RuleArgs a)
 {
-    extern __shared__ uint32_t sm[];
+    extern __shared__ __align__(16) uint32_t sm[];
     uint32_t *key = sm, *count = sm + a.slots;
     float *bias = reinterpret_cast<float *>(sm + 2 * a.slots);
     uint32_t *list = sm + 3 * a.slots;
@@ -197,20 +197,23 @@ template <typename T, bool PIECE> __global__ void __launch_bounds__(kTouchThread
         id0 = blockIdx.x * a.chunk > item.lead ? blockIdx.x * a.chunk - item.lead : 0;
         id1 = item.stop > item.lead ? item.stop - item.lead : 0;
     }
-    // Few enough entries: hashed, in a table of at least 4/3 their number. Else ranges of ids one after the
-    // other, each id at its place.
+    // Few enough entries: hashed, in a table of four times their number where that is smaller than all. Else
+    // ranges of ids one after the other, each id at its place.
     const uint64_t entries = (uint64_t)have + biases;
     const bool hashed = entries <= a.slots / 4 * 3;
     uint32_t slots = a.slots;
     if (hashed)
-        while (slots > 64 && slots / 2 >= entries + entries / 3)
+        while (slots > kLeastSlots && slots / 2 >= 4 * entries)
             slots /= 2;
     bool waited = PIECE;
     for (uint32_t base = id0, width; base < id1; base += width)
     {
         width = hashed ? id1 - base : min(slots, id1 - base); // ids of this round: base .. base + width - 1
-        for (uint32_t i = tid; i < slots; i += threads)
-            key[i] = kNoId, count[i] = 0, bias[i] = 0.f;
+        for (uint32_t i = 4 * tid; i < slots; i += 4 * threads)
+        {
+            *reinterpret_cast<uint4 *>(key + i) = make_uint4(kNoId, kNoId, kNoId, kNoId);
+            *reinterpret_cast<uint4 *>(count + i) = *reinterpret_cast<uint4 *>(bias + i) = make_uint4(0, 0, 0, 0);
+        }
         if (tid == 0)
             listed = 0;
         __syncthreads();
@@ -368,10 +371,11 @@ template <typename T> vkllm_err_t launch_rules(RuleArgs &a, int sms, int device,
             done[device].store(true, std::memory_order_relaxed);
     }
     // One kernel while its blocks run at once: each reads the whole history, but nothing waits for a second
-    // kernel. Of 32000 fp16 logits with up to 768 ids of history, 4 / 32 / 64 / 128 rows take 5.7 / 6.9 /
-    // 11.0 / 16.8 us in one kernel and 9.5 / 10.4 / 10.6 / 11.4 in two; of 32000 fp32 ones with up to 5000
-    // ids, where the large table leaves an SM one block, 16 rows 24.6 and 16.5.
-    if (copy && touch && (uint64_t)a.rows * a.chunks <= (a.slots == kSlotsSmall ? 2 : 1) * (uint64_t)sms)
+    // kernel. Of 32000 fp16 logits with up to 768 ids of history, 4 / 32 / 64 / 128 rows take 4.8 / 5.4 / 9.0 /
+    // 13.3 us in one kernel and 6.4 / 7.0 / 7.2 / 8.2 in two; 16 / 32 rows of 100003 with up to 2048 ids 8.1 /
+    // 13.2 and 10.1 / 10.2; 16 rows of 32000 fp32 ones with up to 5000 ids, where the large table leaves an SM
+    // one block, 19.3 and 16.3.
+    if (copy && touch && (uint64_t)a.rows * a.chunks <= (a.slots == kSlotsSmall ? 3 : 1) * (uint64_t)sms)
     {
         k_logits_touch<T, true><<<dim3(a.chunks, a.rows), kCopyThreads, a.slots * 16, s>>>(a);
         VKB_CUDA(cudaGetLastError());
