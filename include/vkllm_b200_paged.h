@@ -63,7 +63,8 @@ struct vkllm_b200_paged_kv
 {
     void *k, *v; /* device, 16-byte aligned */
     uint64_t page_stride, head_stride, row_stride; /* multiples of 16 bytes */
-    uint32_t n_pages, page_rows, kv_heads;
+    uint32_t n_pages, page_rows; /* n_pages * page_rows < 2^32 */
+    uint32_t kv_heads;           /* <= 65535, as are the query heads, a multiple of them */
     uint32_t head_dim; /* <= 256, head_dim * element size a multiple of 16 */
     uint32_t dtype;    /* vkllm_dtype_float16 or vkllm_dtype_float32: of the pools, q, k, v and out */
     uint32_t reserved; /* 0 */
@@ -94,7 +95,7 @@ extern vkllm_err_t vkllm_b200_paged_append(const struct vkllm_b200_paged_table *
 
 /* Gives the pages of every slot s with done[s] != 0 back to the free list (slot by slot, page by page,
  * onto its top) and sets new_lens[s] to 0; new_lens[s] = lens[s] for the others. All or nothing, as
- * above; the table stays as it is. new_lens may be lens, n_free_out may be n_free. */
+ * above; the table stays as it is. new_lens may be lens, n_free_out may be n_free. n_seqs <= 16384. */
 extern vkllm_err_t vkllm_b200_paged_release(const struct vkllm_b200_paged_table *t, const uint32_t *lens,
                                             const uint32_t *done, const uint32_t *n_free, uint32_t *new_lens,
                                             uint32_t *n_free_out, uint32_t *status, void *stream);

@@ -640,6 +640,35 @@ def test_attention_of_random_shapes(vk, torch, seed):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_of_the_most_sequences(vk, torch, dtype):
+    """65535 slots of none to three rows, a page each: many sequences for every thread of the division, and
+    slots without rows in every CTA's share."""
+    n, hd, R = 65535, 64, 3
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k, v, kv = make_pools(vk, torch, "heads first", n, R, 1, hd, dtype, g)
+    table = torch.randperm(n, generator=g, device="cuda").to(torch.int32).view(n, 1)
+    lens = torch.randint(0, R + 1, (n,), generator=g, device="cuda", dtype=torch.int32)
+    q = torch.randn((n, hd), generator=g, device="cuda").to(k.dtype)
+    out = torch.full_like(q, 7.5)
+    ws, status = torch.zeros(vk.PAGED_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    t = vk.PagedTable(table.data_ptr(), None, 1, n, 1, R, n)
+    assert vk.lib().vkllm_b200_paged_attention(C.byref(kv), C.byref(t), q.data_ptr(), hd, 1, lens.data_ptr(), hd ** -0.5,
+                                               out.data_ptr(), hd, ws.data_ptr(), ws.numel(), status.data_ptr(),
+                                               stream(torch)) == vk.OK
+    torch.cuda.synchronize()
+    assert int(status) == 0
+    K, V = k[table[:, 0].long(), 0].double(), v[table[:, 0].long(), 0].double()
+    sc = (q.double()[:, None] * K).sum(-1) * hd ** -0.5
+    here = torch.arange(R, device="cuda") < lens[:, None]
+    p = torch.where(here, sc, -torch.inf).softmax(-1).nan_to_num(0.0)
+    ref = (p[..., None] * V).sum(1)
+    ds = (hd + 8) * 2 * U * ((q.double()[:, None] * K).abs().sum(-1) * hd ** -0.5).amax(-1)
+    far = (sc.amax(-1) - sc.amin(-1)) * 1.4427
+    tol = (2 * ds + (far + 4 + R + 64) * 2 * U + 2.0 ** -21)[:, None] * (p[..., None] * V.abs()).sum(1) + out_tol(ref, dtype)
+    within(out, ref, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_attention_of_sequences_that_share_pages(vk, torch, dtype):
     """A common beginning held once: both tables name its pages."""
     a = Attend(vk, torch, [100, 90, 70], 8, 2, 64, 16, dtype, seed=31, poison=False)

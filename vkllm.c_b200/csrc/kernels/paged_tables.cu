@@ -17,7 +17,6 @@
 // between the last read and the first write is what makes all-or-nothing and new_lens == lens possible.
 #include <atomic>
 #include <cooperative_groups.h>
-#include <new>
 #include <vector>
 
 #include "paged.cuh"
@@ -479,7 +478,7 @@ extern "C" vkllm_err_t vkllm_b200_paged_check(const struct vkllm_b200_paged_tabl
                 e = take(t->free_pages[j]);
         }
     }
-    catch (const std::bad_alloc &)
+    catch (...)
     {
         return VKLLM_ERR_ALLOC;
     }
