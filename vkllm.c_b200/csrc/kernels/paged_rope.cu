@@ -14,8 +14,9 @@
 //
 // A block works out a token's sines and cosines once, into shared memory; each thread owns one 16-byte
 // piece of a head (4 or 2 pairs), keeps those of its pairs, and walks over its share of the token's heads,
-// 4 loads in flight. 2048 tokens of 40 + 80 heads of 128 (126 MB, fp16): 24.6 us, 5.1 TB/s, where a plain
-// copy of 102 MB reaches 5.5.
+// 4 loads in flight, the first of them on their way before the slot and the sines are known. 2048 tokens of
+// 40 + 80 heads of 128 (126 MB, fp16): 21.8 us, 5.8 TB/s (24.6 with the loads after the sines, 27.5 with
+// sines worked out by every thread), where a plain copy of 102 MB reaches 5.5.
 #include <cmath>
 
 #include "paged.cuh"
@@ -83,37 +84,13 @@ template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_ro
 {
     constexpr int P = Piece<T>::kPairs, E = 2 * P;
     __shared__ __align__(16) float2 table[128]; // (cos, sin) of every pair of a head at the token's position
-    const uint32_t t = blockIdx.x, slot = a.slots[t];
-    if (slot == VKLLM_B200_NO_SLOT)
-        return;
-    const uint32_t page = slot / a.kv.page_rows, row = slot % a.kv.page_rows;
-    if (page >= a.kv.n_pages)
-    {
-        if (threadIdx.x == 0 && blockIdx.y == 0)
-            atomicOr(a.status, (uint32_t)VKLLM_B200_PAGED_BAD_SLOT);
-        return;
-    }
+    const uint32_t t = blockIdx.x, slot = a.slots[t], position = a.positions[t];
     const uint32_t hd = a.kv.head_dim, pieces = hd / E, piece = threadIdx.x % pieces, lanes = blockDim.x / pieces;
-    const uint64_t pos = a.positions[t];
-    for (uint32_t w = threadIdx.x; w < hd / 2; w += blockDim.x)
-    {
-        // half turns in [-1, 1)
-        const float half_turns = __ll2float_rn((long long)(pos * a.turns[w])) * 0x1p-63f;
-        float s, c;
-        sincospif(half_turns, &s, &c);
-        table[w] = make_float2(c, s);
-    }
-    __syncthreads();
-    float cs[P], sn[P];
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-        cs[i] = table[piece * P + i].x, sn[i] = table[piece * P + i].y;
     const uint32_t H = a.heads, K = a.kv.kv_heads, rows = H + 2 * K, off = piece * E;
-    const uint64_t cache = page * a.kv.page_stride + row * a.kv.row_stride + off;
     const uint32_t step = gridDim.y * lanes;
-    for (uint32_t r0 = blockIdx.y * lanes + threadIdx.x / pieces; r0 < rows; r0 += kRopeAhead * step)
-    {
-        uint4 x[kRopeAhead];
+    uint32_t r0 = blockIdx.y * lanes + threadIdx.x / pieces;
+    uint4 x[kRopeAhead];
+    auto load = [&] {
 #pragma unroll
         for (uint32_t u = 0; u < kRopeAhead; ++u)
         {
@@ -125,6 +102,33 @@ template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_ro
                                        : (const T *)a.v + t * a.v_stride + (uint64_t)(r - H - K) * hd;
             x[u] = *reinterpret_cast<const uint4 *>(src + off);
         }
+    };
+    load(); // before the slot and the sines are known: the rows are there for tokens without a slot too
+    if (slot == VKLLM_B200_NO_SLOT)
+        return;
+    const uint32_t page = slot / a.kv.page_rows, row = slot % a.kv.page_rows;
+    if (page >= a.kv.n_pages)
+    {
+        if (threadIdx.x == 0 && blockIdx.y == 0)
+            atomicOr(a.status, (uint32_t)VKLLM_B200_PAGED_BAD_SLOT);
+        return;
+    }
+    for (uint32_t w = threadIdx.x; w < hd / 2; w += blockDim.x)
+    {
+        // half turns in [-1, 1)
+        const float half_turns = __ll2float_rn((long long)(position * a.turns[w])) * 0x1p-63f;
+        float s, c;
+        sincospif(half_turns, &s, &c);
+        table[w] = make_float2(c, s);
+    }
+    __syncthreads();
+    float cs[P], sn[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+        cs[i] = table[piece * P + i].x, sn[i] = table[piece * P + i].y;
+    const uint64_t cache = page * a.kv.page_stride + row * a.kv.row_stride + off;
+    while (r0 < rows)
+    {
 #pragma unroll
         for (uint32_t u = 0; u < kRopeAhead; ++u)
         {
@@ -145,6 +149,8 @@ template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_ro
                                  : (T *)a.kv.v + cache + (r - H - K) * a.kv.head_stride;
             *reinterpret_cast<uint4 *>(dst) = x[u];
         }
+        r0 += kRopeAhead * step;
+        load();
     }
 }
 
@@ -185,8 +191,8 @@ extern "C" vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged
         a.turns[w] = (uint64_t)f;
     const uint32_t pieces = hd * es / 16, threads = kRopeThreads / pieces * pieces, lanes = threads / pieces;
     // Blocks of a token: so many that a thread has one batch of rows in flight (2048 tokens of 120 heads: 2
-    // blocks a token 24.6 us, one 25.9), and of few tokens more, until the call reaches about two blocks an
-    // SM.
+    // blocks a token 24.6 us, one 25.9, when that was measured), and of few tokens more, until the call
+    // reaches about two blocks an SM.
     const uint32_t passes = (heads + 2 * kv->kv_heads + lanes - 1) / lanes;
     uint32_t shares = (passes + kRopeAhead - 1) / kRopeAhead;
     while (shares < passes && (uint64_t)n_tokens * shares < 2u * (uint32_t)sms)
