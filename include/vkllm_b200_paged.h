@@ -131,8 +131,9 @@ extern vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged_kv 
  *          leaves it ready for the next. Calls (and replays of captured calls) that may run at the same
  *          time need a workspace each.
  * A length past cols * page_rows is cut to it and a page id >= n_pages has no keys; both set *status.
- * Sequences may share pages. Scores, softmax and sums are fp32. The same inputs give the same bits on
- * the same device. n_seqs <= 65535. */
+ * Sequences may share pages. Scores, softmax and sums are fp32 (an infinite value among the rows that
+ * count makes its element of out infinite or no number). The same inputs give the same bits on the same
+ * device. n_seqs <= 65535. */
 extern vkllm_err_t vkllm_b200_paged_attention(const struct vkllm_b200_paged_kv *kv,
                                               const struct vkllm_b200_paged_table *t, const void *q, uint64_t q_stride,
                                               uint32_t heads, const uint32_t *lens, float scale, void *out,

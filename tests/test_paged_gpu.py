@@ -640,6 +640,30 @@ def test_attention_of_random_shapes(vk, torch, seed):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_keeps_infinities_where_they_are(vk, torch, dtype):
+    """An infinite value among the rows that count shows in its element of its heads and sequence alone; a key
+    that scores -infinity counts for nothing."""
+    a = Attend(vk, torch, [50, 50], 8, 2, 64, 16, dtype, seed=14)
+    page = int(a.tab[0, 1])
+    a.v[page, 1, 3, 5] = float("inf")
+    a.q[:, :512] = a.q[:, :512].abs() + 0.1
+    a.k[int(a.tab[1, 2]), 0, 7] = -float("inf")  # key 39 of the second sequence, first key head
+    assert a.call() == vk.OK
+    torch.cuda.synchronize()
+    got = a.out[:2, :512].reshape(2, 8, 64)
+    fin = torch.isfinite(got)
+    want = torch.ones_like(fin)
+    want[0, 4:, 5] = False
+    assert torch.equal(fin, want)
+    keep = torch.tensor([j for j in range(50) if j != 39], device="cuda")
+    ids = torch.from_numpy(a.tab[1, :4].astype(np.int64)).cuda()
+    k = a.k[ids].transpose(0, 1).reshape(2, -1, 64)[0, keep].double()
+    v = a.v[ids].transpose(0, 1).reshape(2, -1, 64)[0, keep].double()
+    p = (a.q[1, :256].double().view(4, 64) @ k.T * a.scale).softmax(-1)
+    within(got[1, :4], p @ v, 2.0 ** -11 * (p @ v).abs() + 2.0 ** -16 * (p @ v.abs()) + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_attention_of_the_most_sequences(vk, torch, dtype):
     """65535 slots of none to three rows, a page each: many sequences for every thread of the division, and
     slots without rows in every CTA's share."""
