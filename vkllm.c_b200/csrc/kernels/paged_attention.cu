@@ -499,11 +499,21 @@ template <int KD, int NQ, bool EXACT> struct FloatCore
     __device__ __forceinline__ void start(const PagedAttArgs &a, uint32_t seq, uint32_t head0, uint32_t nq, uint32_t lane,
                                           float *qs)
     {
-        // the CTA's warps are at the same item here: each loads its share of the queries
+        // the CTA's warps are at the same item here: each loads every fourth query, 16 bytes a lane, all in flight
+        // (element by element 118 sequences of up to 13 keys, 64 heads of 128 over 32, took 36.7 us instead of 27.4)
         const uint32_t hd = a.kv.head_dim, warp = threadIdx.x >> 5;
-        for (uint32_t i = warp; i < NQ; i += kWarps)
-            for (uint32_t d = lane; d < KD; d += 32)
-                qs[i * KD + d] = i < nq && d < hd ? ((const T *)a.q)[seq * a.q_stride + (uint64_t)(head0 + i) * hd + d] : 0.f;
+        const T *q = (const T *)a.q + seq * a.q_stride + (uint64_t)head0 * hd;
+#pragma unroll
+        for (uint32_t j = 0; j < (NQ + kWarps - 1) / kWarps; ++j)
+#pragma unroll
+            for (uint32_t k = 0; k < kOwn; ++k)
+            {
+                const uint32_t i = warp + kWarps * j, d = 4 * (lane + 32 * k);
+                if (i < NQ && d < KD)
+                    reinterpret_cast<float4 *>(qs)[(i * KD + d) / 4] =
+                        i < nq && (EXACT || d < hd) ? __ldg(reinterpret_cast<const float4 *>(q + i * hd + d))
+                                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
