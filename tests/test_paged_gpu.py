@@ -275,6 +275,49 @@ def test_release_is_all_or_nothing(vk, torch, what, bit):
     b.same(got, (b.lens, b.count))
 
 
+@pytest.mark.parametrize("n", [65, 129, 1100, 2100])
+def test_tables_beside_other_work(vk, torch, n):
+    """Clusters of 2 to 8 CTAs (release: 65, 129 and more slots; append: 1100 and 2100) while products on another
+    stream leave SMs free a few at a time, so that a cluster's CTAs start when they can. Their words about bad
+    values have to reach every one of them: each round has one call that has to be refused by all."""
+    b = Book(vk, torch, [4] * n, 6, 4, spare=2 * n, seed=n)
+    other, x = torch.cuda.Stream(), torch.randn(4096, 4096, device="cuda").half()
+    torch.cuda.synchronize()
+    done = np.zeros(n, dtype=np.uint32)
+    done[::3] = 1
+    for i in range(12):
+        with torch.cuda.stream(other):
+            for _ in range(4):
+                x @ x
+        b.same(b.append([1] * n, n + 5), b.want_append([1] * n, n + 5)[0])
+        assert int(u32(b.status)[0]) == 0
+        # a bad page of one sequence, found by one CTA alone
+        s = int(np.flatnonzero(done)[-1 - i % 3])
+        keep, b.table[s, 1] = b.table[s, 1], b.n_pages
+        b.d_table.copy_(i32(torch, b.table))
+        with torch.cuda.stream(other):
+            x @ x
+        for call in (lambda: b.release(done), lambda: b.append([1] * n, n)):
+            got = call()
+            assert int(u32(b.status)[0]) == vk.PAGED_BAD_PAGE
+            assert np.array_equal(got[0], b.lens) and got[1] == b.count
+            b.status.zero_()
+        assert np.array_equal(u32(b.d_table), b.table) and np.array_equal(u32(b.d_free), b.free)
+        b.table[s, 1] = keep
+        b.d_table.copy_(i32(torch, b.table))
+        b.same(b.release(done), b.want_release(done))
+        new = np.where(done != 0, 4, 0)
+        b.same(b.append(new, 4 * n), b.want_append(new, 4 * n)[0])
+        b.lens[:] = np.where(done != 0, b.lens, 4)  # the others' second pages go back to the list by hand
+        held = b.table[done == 0, 1]
+        b.free[b.count:b.count + len(held)], b.count = held, b.count + len(held)
+        b.d_lens.copy_(i32(torch, b.lens))
+        b.d_free.copy_(i32(torch, b.free))
+        b.d_count.copy_(i32(torch, [b.count]))
+        assert int(u32(b.status)[0]) == 0
+    torch.cuda.synchronize()
+
+
 # ---- pools ---------------------------------------------------------------------------------------
 
 LAYOUTS = ["heads first", "rows first", "joined"]

@@ -14,7 +14,8 @@
 // over the GPU). Every CTA sums all sequences itself (they are few; a scan split over CTAs would need an
 // exchange more) into shared memory, then takes its share of the tokens, pages and sequences, found by
 // binary search in the sums, so one long prompt among many short ones spreads evenly. The cluster barrier
-// between the last read and the first write is what makes all-or-nothing and new_lens == lens possible.
+// between the last read and the first write is what makes all-or-nothing and new_lens == lens possible. The
+// CTAs say at their start that they run: only then may another one write their shared memory.
 #include <atomic>
 #include <cooperative_groups.h>
 #include <vector>
@@ -106,13 +107,20 @@ __device__ void block_sums(uint64_t &a, uint64_t &b, uint64_t *ta, uint64_t *tb)
 }
 
 // The OR of every CTA's `err` (shared memory) over the cluster, and a barrier between the reads before
-// and the writes after it.
+// and the writes after it. Every thread of the cluster has to have arrived at the cluster's barrier once
+// before (cluster_started): a CTA's shared memory may be written by others from its start on only, and the
+// wait here, which the sums have mostly hidden, is what says that all have started.
+__device__ __forceinline__ void cluster_started()
+{
+    cooperative_groups::this_cluster().barrier_arrive();
+}
 __device__ uint32_t cluster_or(uint32_t *err)
 {
     namespace cg = cooperative_groups;
     cg::cluster_group cl = cg::this_cluster();
     __shared__ uint32_t all[kMaxCluster];
     __syncthreads(); // err is final in this CTA
+    cl.barrier_wait();
     if (threadIdx.x < cl.num_blocks())
         *cl.map_shared_rank(&all[cl.block_rank()], threadIdx.x) = *err;
     cl.sync();
@@ -129,6 +137,7 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_append(const AppendArgs a
     __shared__ uint32_t err;
     const uint32_t n = a.t.n_seqs, R = a.t.page_rows, tid = threadIdx.x;
     const uint32_t rank = cg::this_cluster().block_rank(), size = cg::this_cluster().num_blocks();
+    cluster_started();
     uint32_t *starts = sm, *first = sm + n + 1, *len = first + n + 1; // [n + 1], [n + 1], [n]
     const uint32_t nf = *a.n_free;
     if (tid == 0)
@@ -289,6 +298,7 @@ __global__ void __launch_bounds__(kTabThreads) k_paged_release(const ReleaseArgs
     __shared__ uint32_t err;
     const uint32_t n = a.t.n_seqs, R = a.t.page_rows, tid = threadIdx.x;
     const uint32_t rank = cg::this_cluster().block_rank(), size = cg::this_cluster().num_blocks();
+    cluster_started();
     uint32_t *first = sm, *len = sm + n + 1; // [n + 1], [n]
     const uint32_t nf = *a.n_free;
     if (tid == 0)
