@@ -448,6 +448,41 @@ def test_rope_write_flags_a_slot_outside_the_pool(vk, torch):
     assert sorted((p * 8 + r) for p, r in changed.nonzero().tolist()) == [1, 5, 23]
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_rope_write_of_padding_does_not_read_its_rows(vk, torch, dtype):
+    """64 tokens in a launch for 16384, as a captured step for the most tokens has it: it costs what the slots and
+    the launch cost, not the traffic of rows that no slot wants. Rows read for nothing would take 14 us (fp16; 100 MB
+    at 7 TB/s) beyond that, so a third of the full call's time is a bound that only reading them passes."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    H, HK, hd, n, R = 16, 4, 128, 16384, 64
+    if dtype == "f16":
+        H, HK = 32, 8
+    k, v, kv = make_pools(vk, torch, "heads first", n // R, R, HK, hd, dtype, g)
+    qkv = torch.randn((n, (H + 2 * HK) * hd), generator=g, device="cuda").to(k.dtype)
+    q_out = torch.zeros((n, H * hd), dtype=k.dtype, device="cuda")
+    full = torch.randperm(n, generator=g, device="cuda").to(torch.int32)
+    few = full.clone()
+    few[64:] = -1
+    pos, status = torch.arange(n, device="cuda", dtype=torch.int32), torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def best(slots):
+        times = []
+        for _ in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(5):
+                assert rope_call(vk, torch, kv, qkv, H, HK, hd, pos, slots, n, 0.0, q_out, status) == vk.OK
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times[2:])
+
+    q_out.zero_()
+    padded = best(few)
+    assert bool((q_out[64:] == 0).all()) and bool((q_out[:64] != 0).any())
+    assert padded < best(full) / 3 and int(status) == 0
+
+
 # ---- attention -----------------------------------------------------------------------------------
 
 class Attend:

@@ -14,9 +14,14 @@
 //
 // A block works out a token's sines and cosines once, into shared memory; each thread owns one 16-byte
 // piece of a head (4 or 2 pairs), keeps those of its pairs, and walks over its share of the token's heads,
-// 4 loads in flight, the first of them on their way before the slot and the sines are known. 2048 tokens of
-// 40 + 80 heads of 128 (126 MB, fp16): 21.8 us, 5.8 TB/s (24.6 with the loads after the sines, 27.5 with
-// sines worked out by every thread), where a plain copy of 102 MB reaches 5.5.
+// kAhead loads in flight, the first of them on their way before the position and the sines are known. 2048
+// tokens of 40 + 80 heads of 128 (126 MB, fp16): 20.4 us, 6.2 TB/s (24.6 with the loads after the sines, 27.5
+// with sines worked out by every thread), where a plain copy of 102 MB reaches 5.5.
+//
+// The loads wait for the slot: a step that is launched for the most tokens it may have is mostly padding, whose
+// rows are not read. 64 tokens among 8192, 32 + 16 heads of 128: 5.5 us; 20.6 where the loads go out first, which
+// gives 64 tokens without padding 2.6 us instead of 2.7, 2048 of 32 + 16 heads 10.2 instead of 10.5 and longer
+// calls nothing.
 #include <cmath>
 
 #include "paged.cuh"
@@ -28,7 +33,6 @@ namespace
 {
 
 constexpr uint32_t kRopeThreads = 256;
-constexpr uint32_t kRopeAhead = 4; // rows of a thread in flight
 
 struct RopeArgs
 {
@@ -42,10 +46,14 @@ struct RopeArgs
     uint64_t turns[128]; // base^(-2w / hd) / (2 pi) * 2^64
 };
 
-template <typename T> struct Piece; // 16 bytes as fp32 pairs
+// 16 bytes as fp32 pairs. kAhead: rows of a thread in flight; kCtas: blocks of an SM that the registers are kept
+// to. fp16 2048 tokens of 40 + 80 heads take 20.4 us with 4 x 6 blocks, 21.5 with 4 x 5, 21.8 with 3 x 8, 23.1 with
+// 4 x 8 (registers spill); fp32 1500 tokens of 32 + 16 heads 12.5 with 3 x 8, 13.4 with 4 x 6.
+template <typename T> struct Piece;
 template <> struct Piece<__half>
 {
     static constexpr int kPairs = 4;
+    static constexpr uint32_t kAhead = 4, kCtas = 6;
     __device__ static void load(const uint4 &r, float2 (&p)[4])
     {
         const __half2 *h = reinterpret_cast<const __half2 *>(&r);
@@ -66,6 +74,7 @@ template <> struct Piece<__half>
 template <> struct Piece<float>
 {
     static constexpr int kPairs = 2;
+    static constexpr uint32_t kAhead = 3, kCtas = 8;
     __device__ static void load(const uint4 &r, float2 (&p)[2])
     {
         p[0] = make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
@@ -80,19 +89,21 @@ template <> struct Piece<float>
 
 // Block: a multiple of the pieces of a head; grid.x: tokens, grid.y: shares of the token's rows (q heads,
 // then key heads, then value heads).
-template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_rope_write(const RopeArgs a)
+template <typename T>
+__global__ void __launch_bounds__(kRopeThreads, Piece<T>::kCtas) k_paged_rope_write(const RopeArgs a)
 {
     constexpr int P = Piece<T>::kPairs, E = 2 * P;
+    constexpr uint32_t kAhead = Piece<T>::kAhead;
     __shared__ __align__(16) float2 table[128]; // (cos, sin) of every pair of a head at the token's position
-    const uint32_t t = blockIdx.x, slot = a.slots[t], position = a.positions[t];
+    const uint32_t t = blockIdx.x, slot = a.slots[t];
     const uint32_t hd = a.kv.head_dim, pieces = hd / E, piece = threadIdx.x % pieces, lanes = blockDim.x / pieces;
     const uint32_t H = a.heads, K = a.kv.kv_heads, rows = H + 2 * K, off = piece * E;
     const uint32_t step = gridDim.y * lanes;
     uint32_t r0 = blockIdx.y * lanes + threadIdx.x / pieces;
-    uint4 x[kRopeAhead];
+    uint4 x[kAhead];
     auto load = [&] {
 #pragma unroll
-        for (uint32_t u = 0; u < kRopeAhead; ++u)
+        for (uint32_t u = 0; u < kAhead; ++u)
         {
             const uint32_t r = r0 + u * step;
             if (r >= rows)
@@ -103,9 +114,10 @@ template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_ro
             x[u] = *reinterpret_cast<const uint4 *>(src + off);
         }
     };
-    load(); // before the slot and the sines are known: the rows are there for tokens without a slot too
     if (slot == VKLLM_B200_NO_SLOT)
         return;
+    load();
+    const uint32_t position = a.positions[t]; // (read with the slot, it would be waited for with it)
     const uint32_t page = slot / a.kv.page_rows, row = slot % a.kv.page_rows;
     if (page >= a.kv.n_pages)
     {
@@ -130,7 +142,7 @@ template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_ro
     while (r0 < rows)
     {
 #pragma unroll
-        for (uint32_t u = 0; u < kRopeAhead; ++u)
+        for (uint32_t u = 0; u < kAhead; ++u)
         {
             const uint32_t r = r0 + u * step;
             if (r >= rows)
@@ -149,7 +161,7 @@ template <typename T> __global__ void __launch_bounds__(kRopeThreads) k_paged_ro
                                  : (T *)a.kv.v + cache + (r - H - K) * a.kv.head_stride;
             *reinterpret_cast<uint4 *>(dst) = x[u];
         }
-        r0 += kRopeAhead * step;
+        r0 += kAhead * step;
         load();
     }
 }
@@ -193,8 +205,9 @@ extern "C" vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged
     // Blocks of a token: so many that a thread has one batch of rows in flight (2048 tokens of 120 heads: 2
     // blocks a token 24.6 us, one 25.9, when that was measured), and of few tokens more, until the call
     // reaches about two blocks an SM.
+    const uint32_t ahead = es == 2 ? Piece<__half>::kAhead : Piece<float>::kAhead;
     const uint32_t passes = (heads + 2 * kv->kv_heads + lanes - 1) / lanes;
-    uint32_t shares = (passes + kRopeAhead - 1) / kRopeAhead;
+    uint32_t shares = (passes + ahead - 1) / ahead;
     while (shares < passes && (uint64_t)n_tokens * shares < 2u * (uint32_t)sms)
         ++shares;
     const dim3 grid(n_tokens, shares);
