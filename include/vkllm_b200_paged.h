@@ -154,7 +154,7 @@ struct vkllm_b200_logit_rules
     const uint32_t *bias_ids;     /* x + value; an id listed twice gets both, in the order of the list */
     const float *bias_values;
     const uint32_t *mask;         /* bit id % 32 of word id / 32 of a row: 0 makes the logit -infinity */
-    uint64_t history_stride, mask_stride; /* elements and words from row to row */
+    uint64_t history_stride, mask_stride; /* elements and words from row to row; history_stride < 2^30 */
 };
 
 /* out = logits under the rules, in the order of the struct (repetition, frequency and presence, biases,

@@ -141,6 +141,12 @@ def test_logit_rules_refused(vk, bad):
     assert apply(vk, None) == vk.ARGS
 
 
+@pytest.mark.parametrize("stride", [1 << 30, (1 << 32) - 1, 1 << 39])
+def test_logit_rules_refuse_histories_past_30_bits(vk, stride):
+    """An id's count has 30 bits beside two marks, and a history of nearly 2^32 ids would wrap the 32-bit places."""
+    assert apply(vk, rules(vk, history=P, history_lens=P, history_stride=stride)) == vk.ARGS
+
+
 # ---- vkllm_b200_paged_check ----------------------------------------------------------------------
 
 def check(vk, tab, lens, free=(), page_rows=4, n_pages=10, n_free=None):

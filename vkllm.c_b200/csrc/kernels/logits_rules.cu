@@ -39,6 +39,9 @@ constexpr uint32_t kTouchThreads = 512; // of a row, or half as many where rows 
 constexpr uint32_t kSlotsSmall = 4096, kSlotsLarge = 8192, kLeastSlots = 512;
 constexpr uint32_t kNoId = 0xffffffffu; // not an id: vocab < 2^31
 constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u; // in the prompt; in the biases; the bits below: times generated
+// Ids of a history are fewer: an id's count stays below kBiased, and places in a history do not wrap in 32 bits
+// where a thread looks a few thousand ahead.
+constexpr uint64_t kMostHistory = kBiased;
 
 struct RuleArgs
 {
@@ -423,7 +426,7 @@ extern "C" vkllm_err_t vkllm_b200_logits_apply(const struct vkllm_b200_logit_rul
                 aligned_to(rules->presence, 4));
     _CHECK_ARGS(!rules->bias_starts || (words(rules->bias_starts) && words(rules->bias_ids) && words(rules->bias_values)));
     _CHECK_ARGS(!rules->mask || (words(rules->mask) && rules->mask_stride >= ((uint64_t)vocab + 31) / 32));
-    _CHECK_ARGS(rules->history_stride < (1ull << 40) && rules->mask_stride < (1ull << 40));
+    _CHECK_ARGS((!rules->history || rules->history_stride < kMostHistory) && rules->mask_stride < (1ull << 40));
     int sms = 0, dev = 0;
     const vkllm_b200_logit_rules &r = *rules;
     _CHECK(check_device({logits, out, r.history, r.history ? r.prompt_lens : nullptr, r.history ? r.history_lens : nullptr, r.repetition,
