@@ -792,6 +792,50 @@ def test_attention_says_when_its_workspace_was_not_zero(vk, torch):
     a.check()
 
 
+def test_an_error_of_one_call_is_not_told_again_by_the_next(vk, torch, ctx):
+    """A call on the legacy stream while another, blocking stream is being captured is an error of CUDA's (and ends
+    that capture). The calls after it are right and say so, the graph ops among them."""
+    a = Attend(vk, torch, [20, 3], 2, 2, 64, 16, "f16")
+    b = Book(vk, torch, [3], 4, 4, spare=3)
+    qkv, q_out = torch.ones((2, 6 * 64), dtype=torch.float16, device="cuda"), a.out.clone()
+    pos = i32(torch, [0, 1])
+    slots = i32(torch, [0xffffffff, 0xffffffff])
+    x = torch.randn((2, 64), device="cuda").half()
+    y, rule = torch.zeros_like(x), vk.LogitRules()
+    t = vk.tensor_new(ctx, "x", (1, 1, 2, 64), vk.F16)
+    vk.put(ctx, t, np.arange(128, dtype=np.float16).reshape(1, 1, 2, 64))
+    torch.cuda.synchronize()
+    cuda = C.CDLL("libcuda.so.1")
+
+    def fail():
+        s, g = C.c_void_p(), C.c_void_p()
+        assert cuda.cuStreamCreate(C.byref(s), 0) == 0  # blocking: ordered with the legacy stream
+        assert cuda.cuStreamBeginCapture_v2(s, 2) == 0
+        err = vk.lib().vkllm_b200_paged_release(C.byref(b.c_table()), b.d_lens.data_ptr(), b.d_lens.data_ptr(),
+                                                b.d_count.data_ptr(), b.d_lens.data_ptr(), b.d_count.data_ptr(),
+                                                b.status.data_ptr(), None)
+        cuda.cuStreamEndCapture(s, C.byref(g))
+        assert cuda.cuStreamDestroy_v2(s) == 0
+        return err
+
+    own = torch.cuda.Stream()
+    with torch.cuda.stream(own):
+        for call in (lambda: rope_call(vk, torch, a.kv, qkv, 2, 2, 64, pos, slots, 2, 0.0, q_out, a.status), a.call,
+                     lambda: vk.lib().vkllm_b200_logits_apply(C.byref(rule), x.data_ptr(), 64, 2, 64, vk.F16, y.data_ptr(), 64,
+                                                              own.cuda_stream)):
+            assert fail() == vk.VULKAN
+            assert call() == vk.OK
+    assert fail() == vk.VULKAN
+    node = vk.tensor_new(ctx, "token", (1, 1, 2, 1), vk.U32, op=vk.OP_ARG_MAX, srcs=[t], mapped=True)
+    vk.run_op(ctx, node, "vkllm_op_arg_max_init", "vkllm_op_arg_max_run")
+    assert vk.fetch(ctx, node).reshape(-1).tolist() == [63, 63]
+    torch.cuda.synchronize()
+    a.check()
+    assert torch.equal(y, x) and int(b.d_lens) == 3
+    vk.tensor_free(ctx, node)
+    vk.tensor_free(ctx, t)
+
+
 FIRST_CALLS = """
 import ctypes as C, sys
 sys.path[:0] = [{pkg!r}]

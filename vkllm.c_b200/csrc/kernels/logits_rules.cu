@@ -379,16 +379,11 @@ template <typename T> vkllm_err_t launch_rules(RuleArgs &a, int sms, int device,
     // 13.2 and 10.1 / 10.2; 16 rows of 32000 fp32 ones with up to 5000 ids, where the large table leaves an SM
     // one block, 19.3 and 16.3.
     if (copy && touch && (uint64_t)a.rows * a.chunks <= (a.slots == kSlotsSmall ? 3 : 1) * (uint64_t)sms)
-    {
-        k_logits_touch<T, true><<<dim3(a.chunks, a.rows), kCopyThreads, a.slots * 16, s>>>(a);
-        VKB_CUDA(cudaGetLastError());
-        return VKLLM_ERR_OK;
-    }
+        return launch_plain(k_logits_touch<T, true>, a, dim3(a.chunks, a.rows), kCopyThreads, a.slots * 16, s);
     if (copy)
     {
         const uint64_t items = (uint64_t)a.rows * a.chunks, most = (uint64_t)sms * kCopyCtas;
-        k_logits_copy<T><<<(unsigned)(items < most ? items : most), kCopyThreads, 0, s>>>(a);
-        VKB_CUDA(cudaGetLastError());
+        _CHECK(launch_plain(k_logits_copy<T>, a, dim3((unsigned)(items < most ? items : most)), kCopyThreads, 0, s));
     }
     if (!touch)
         return VKLLM_ERR_OK;

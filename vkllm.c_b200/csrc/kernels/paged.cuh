@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <initializer_list>
 
+#include "../runtime/internal.h"
 #include "common.cuh"
 #include "vkllm_b200_paged.h"
 #include "vkllm_common.h"
@@ -66,6 +67,21 @@ inline bool words(const void *p)
 // (null pointers are passed over). *sms receives the SM count of the current device. Looking at a pointer
 // takes the host 50 ns.
 vkllm_err_t check_device(std::initializer_list<const void *> arrays, int *sms, int *device);
+
+// Launches a kernel without attributes and returns its own status: cudaGetLastError after <<<>>> would also tell of
+// errors of earlier calls.
+template <typename Args>
+vkllm_err_t launch_plain(void (*kernel)(const Args), const Args &args, dim3 grid, uint32_t threads, size_t smem,
+                         cudaStream_t s)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    VKB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
+    return VKLLM_ERR_OK;
+}
 
 // A table whose shape fits (the pointers' targets are not looked at).
 inline bool table_fits(const vkllm_b200_paged_table *t)

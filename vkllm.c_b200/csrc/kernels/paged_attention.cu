@@ -986,9 +986,7 @@ vkllm_err_t launch(PagedAttArgs &a, int sms, int device, cudaStream_t s)
     grid = grid < work ? grid : work;
     grid = grid < room ? grid : room;
     grid = grid < kCounters ? grid : kCounters;
-    kernel<<<(unsigned)grid, kThreads, S::kSmem, s>>>(a);
-    VKB_CUDA(cudaGetLastError());
-    return VKLLM_ERR_OK;
+    return launch_plain(kernel, a, dim3((unsigned)grid), kThreads, S::kSmem, s);
 }
 
 template <template <int, int, bool> class Kind, typename T, int KD, int NQ>

@@ -211,10 +211,6 @@ extern "C" vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged
     while (shares < passes && (uint64_t)n_tokens * shares < 2u * (uint32_t)sms)
         ++shares;
     const dim3 grid(n_tokens, shares);
-    if (kv->dtype == vkllm_dtype_float16)
-        k_paged_rope_write<__half><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
-    else
-        k_paged_rope_write<float><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
-    VKB_CUDA(cudaGetLastError());
-    return VKLLM_ERR_OK;
+    return launch_plain(kv->dtype == vkllm_dtype_float16 ? k_paged_rope_write<__half> : k_paged_rope_write<float>, a, grid,
+                        threads, 0, (cudaStream_t)stream);
 }

@@ -116,6 +116,7 @@ void CachingAllocator::trim()
 vkllm_err_t cuda_check(cudaError_t e, const char *what, const char *file, int line)
 {
     vkllm_log(VKLLM_LOG_ERROR, file, line, "%s failed: %s (%d)", what, cudaGetErrorString(e), (int)e);
+    (void)cudaGetLastError(); // reported here: a later call that checks its launch must not find it again
     return VKLLM_ERR_VULKAN;
 }
 
