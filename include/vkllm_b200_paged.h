@@ -1,5 +1,5 @@
 /* Serving operators over a paged KV cache: page tables and slot maps built on the GPU, RoPE with the
- * key and value rows written into the pages, attention of one new token per sequence over them, and
+ * key and value rows written into the pages, attention of one query row per table row over them, and
  * penalties, biases and grammar masks on the logits. None has a counterpart in the reference, whose KV
  * cache is one contiguous tensor per layer (src/models/vkllm_kvcache.c) and whose token choice is a
  * plain argmax.
@@ -119,14 +119,17 @@ extern vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged_kv 
 /* Size of the workspace that vkllm_b200_paged_attention asks for (the same for every shape). */
 #define VKLLM_B200_PAGED_WORKSPACE_BYTES (16u << 20)
 
-/* Attention of one new token per sequence slot: out = softmax(scale q . K) V over the lens[s] cached rows
- * of slot s, whose query is the token of the last of them; query head h reads key head
- * h / (heads / kv_heads). This is plain attention at every length (unlike VKLLM_OP_MATMUL, nothing
- * depends on lens[s] == head_dim).
+/* Attention of one query row per row of the table: out = softmax(scale q . K) V over the lens[s] cached
+ * rows of table row s, for the query in row s of q; query head h reads key head h / (heads / kv_heads). This
+ * is plain attention at every length (unlike VKLLM_OP_MATMUL, nothing depends on lens[s] == head_dim).
  *   q, out [n_seqs] rows of heads * head_dim, row strides in elements (multiples of 16 bytes, pointers
  *          16-byte aligned), of the pools' type; out must not overlap q
- *   lens   [n_seqs]; a slot with 0 rows, or whose every score is -infinity, gets a row of zeros; rows of
- *          the cache past lens[s] have no effect whatever they hold (no number, infinities)
+ *   lens   [n_seqs]; a row with 0 rows of cache, or whose every score is -infinity, gets a row of zeros; rows
+ *          of the cache past lens[s] have no effect whatever they hold (no number, infinities)
+ * Row s of q goes with row s of the table and nothing else: the table of the sequence slots fits the packed
+ * rows of vkllm_b200_paged_append and _rope_write only in a step with exactly one new token in every slot. For
+ * any other step (slots without a new token, prompts) the call takes a table of its own, a row per packed
+ * token: row i a copy of its slot's row, lens[i] = positions[i] + 1 (so a prompt is causal), 0 past the last.
  *   workspace  16-byte aligned, VKLLM_B200_PAGED_WORKSPACE_BYTES, zero before its first use; every call
  *          leaves it ready for the next. Calls (and replays of captured calls) that may run at the same
  *          time need a workspace each.
