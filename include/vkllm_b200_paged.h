@@ -46,7 +46,12 @@ enum
 };
 
 /* The page table of a batch of sequence slots. Row s of a sequence's cache is row s % page_rows of page
- * table[seq * stride + s / page_rows]. */
+ * table[seq * stride + s / page_rows].
+ * Every page of a table that vkllm_b200_paged_append or _release gets, and of its free list, is held once.
+ * vkllm_b200_paged_check finds a page that is held twice; the calls on the device do not look for one. They
+ * would hand it out while the other holder still reads it, or twice, or let both write its rows. Pages are
+ * shared in tables that only the attention gets, whose rows name pages of such a table's sequences; a
+ * sequence outlives those that read its pages. */
 struct vkllm_b200_paged_table
 {
     uint32_t *table;      /* device, [n_seqs] rows of cols page ids */
@@ -84,8 +89,9 @@ extern vkllm_err_t vkllm_b200_paged_check(const struct vkllm_b200_paged_table *t
  *   slots     [max_tokens] receives page * page_rows + row of each token, VKLLM_B200_NO_SLOT past the last
  *   positions [max_tokens] receives each token's position in its sequence, 0 past the last
  * Pages come off the top of the free list, slot by slot and in order, and are written behind the ones
- * in the table; the rest of the table stays as it is. All or nothing: when a length, the free list or
- * max_tokens does not allow it, *status says so and the call does what it would do for n_new all 0.
+ * in the table (none of which two slots may hold); the rest of the table stays as it is. All or nothing:
+ * when a length, the free list or max_tokens does not allow it, *status says so and the call does what it
+ * would do for n_new all 0.
  * new_lens may be lens and n_free_out may be n_free (advance in place); other arrays must not overlap.
  * n_seqs <= 16384. max_tokens may be 0 (slots and positions may then be NULL). */
 extern vkllm_err_t vkllm_b200_paged_append(const struct vkllm_b200_paged_table *t, const uint32_t *lens,
@@ -93,9 +99,10 @@ extern vkllm_err_t vkllm_b200_paged_append(const struct vkllm_b200_paged_table *
                                            uint32_t *n_free_out, uint32_t *starts, uint32_t *slots, uint32_t *positions,
                                            uint32_t max_tokens, uint32_t *status, void *stream);
 
-/* Gives the pages of every slot s with done[s] != 0 back to the free list (slot by slot, page by page,
- * onto its top) and sets new_lens[s] to 0; new_lens[s] = lens[s] for the others. All or nothing, as
- * above; the table stays as it is. new_lens may be lens, n_free_out may be n_free. n_seqs <= 16384. */
+/* Gives the pages of every slot s with done[s] != 0 (none of which another slot may hold) back to the free
+ * list, slot by slot, page by page, onto its top, and sets new_lens[s] to 0; new_lens[s] = lens[s] for the
+ * others. All or nothing, as above; the table stays as it is. new_lens may be lens, n_free_out may be n_free.
+ * n_seqs <= 16384. */
 extern vkllm_err_t vkllm_b200_paged_release(const struct vkllm_b200_paged_table *t, const uint32_t *lens,
                                             const uint32_t *done, const uint32_t *n_free, uint32_t *new_lens,
                                             uint32_t *n_free_out, uint32_t *status, void *stream);
@@ -134,7 +141,8 @@ extern vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged_kv 
  *          leaves it ready for the next. Calls (and replays of captured calls) that may run at the same
  *          time need a workspace each.
  * A length past cols * page_rows is cut to it and a page id >= n_pages has no keys; both set *status.
- * Sequences may share pages. Scores, softmax and sums are fp32 (an infinite value among the rows that
+ * Rows of the table may share pages (a table of the attention's own, not one that append and release keep:
+ * see struct vkllm_b200_paged_table). Scores, softmax and sums are fp32 (an infinite value among the rows that
  * count makes its element of out infinite or no number). The same inputs give the same bits on the same
  * device. n_seqs <= 65535. */
 extern vkllm_err_t vkllm_b200_paged_attention(const struct vkllm_b200_paged_kv *kv,

@@ -780,6 +780,55 @@ def test_attention_of_sequences_that_share_pages(vk, torch, dtype):
     a.check()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_a_shared_beginning_outlives_release_and_append(vk, torch, dtype):
+    """A common beginning of three pages is held by one slot; the others hold what is their own, and a table of the
+    attention's own names the beginning's pages before theirs. Readers end, others come: nothing of the beginning
+    is handed out, and the slots' table stays consistent. The joint table itself is refused by the check."""
+    H, HK, hd, R, n, cols = 8, 2, 64, 16, 4, 5
+    a = Attend(vk, torch, [48, 20, 33, 7], H, HK, hd, R, dtype, seed=41, poison=False, cols=cols)
+    lens, own = [48, 20, 33, 7], a.tab[:, :cols].copy()
+    spare = sorted(set(range(a.n_pages)) - {int(p) for s in range(n) for p in own[s, :-(-lens[s] // R)]})
+    a.k.copy_(torch.randn(a.k.shape, device="cuda"))
+    a.v.copy_(torch.randn(a.v.shape, device="cuda"))
+    beginning = own[0, :3].copy()
+    d_own, d_lens, count = i32(torch, own), i32(torch, lens), i32(torch, [len(spare)])
+    free = i32(torch, spare + [0xeeeeeeee] * (a.n_pages - len(spare)))
+    t = vk.PagedTable(d_own.data_ptr(), free.data_ptr(), cols, n, cols, R, a.n_pages)
+    z = lambda m: torch.zeros(m, dtype=torch.int32, device="cuda")  # noqa: E731
+    starts, slots, pos = z(n + 1), z(16), z(16)
+    p = lambda x: x.data_ptr()  # noqa: E731
+
+    def check(table, ln, some):
+        ht = vk.PagedTable(table.ctypes.data, some.ctypes.data, table.shape[1], n, cols + 3, R, a.n_pages)
+        return vk.lib().vkllm_b200_paged_check(C.byref(ht), ln.ctypes.data, len(some), None, None)
+
+    for done, new in (([0] * n, [0, 1, 1, 1]), ([0, 1, 0, 0], [0, 9, 0, 1]), ([0, 0, 1, 1], [0, 1, 5, 2])):
+        assert vk.lib().vkllm_b200_paged_release(C.byref(t), p(d_lens), p(i32(torch, done)), p(count), p(d_lens), p(count),
+                                                 p(a.status), stream(torch)) == vk.OK
+        assert vk.lib().vkllm_b200_paged_append(C.byref(t), p(d_lens), p(i32(torch, new)), p(count), p(d_lens), p(count), p(starts),
+                                                p(slots), p(pos), 16, p(a.status), stream(torch)) == vk.OK
+        torch.cuda.synchronize()
+        lens = [0 if d else l for l, d in zip(lens, done)]
+        lens = [l + m for l, m in zip(lens, new)]
+        own = u32(d_own).copy()
+        assert int(a.status) == 0 and u32(d_lens).tolist() == lens and (own[0, :3] == beginning).all()
+        left = u32(free)[:int(count)].copy()
+        assert not set(beginning.tolist()) & set(left.tolist())
+        wide = np.full((n, cols + 3), 0xffffffff, dtype=np.uint32)
+        wide[:, :cols] = own
+        assert check(wide, np.asarray(lens, dtype=np.uint32), left) == vk.OK
+        a.tab = np.full((n, cols + 3), 0xffffffff, dtype=np.uint32)
+        a.tab[0, :cols], a.tab[1:, :3], a.tab[1:, 3:] = own[0], beginning, own[1:]
+        a.lens = [lens[0]] + [48 + l for l in lens[1:]]
+        assert check(a.tab, np.asarray(a.lens, dtype=np.uint32), left) == vk.ARGS
+        a.d_tab, a.d_lens = i32(torch, a.tab), i32(torch, a.lens)
+        a.table = vk.PagedTable(p(a.d_tab), None, cols + 3, n, cols + 3, R, a.n_pages)
+        a.out.fill_(7.5)
+        assert a.call() == vk.OK
+        a.check()
+
+
 def test_attention_says_when_its_workspace_was_not_zero(vk, torch):
     a = Attend(vk, torch, [40000], 8, 2, 64, 16, "f16")
     a.ws.fill_(255)
