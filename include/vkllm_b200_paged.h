@@ -16,7 +16,8 @@
  * nothing was enqueued. VKLLM_ERR_VULKAN: a CUDA error.
  * Lengths, counts, page ids and slots in device memory that do not fit are found by the kernels: they
  * set bits of the device word *status (zeroed by the caller, only ever OR-ed into) and lead to no access
- * outside the arrays. */
+ * outside the arrays. One thing on the device they cannot check, since no length is given for it: the entries
+ * of bias_starts in struct vkllm_b200_logit_rules have to lie within the two lists. */
 #ifndef VKLLM_B200_PAGED_H
 #define VKLLM_B200_PAGED_H
 
@@ -161,8 +162,10 @@ struct vkllm_b200_logit_rules
     const float *frequency;       /* [rows]: x - frequency * (times generated) */
     const float *presence;        /* [rows]: x - presence for ids generated at least once */
     const uint32_t *bias_starts;  /* [rows + 1], ascending: row r's biases are entries bias_starts[r] up to
-                                   * bias_starts[r + 1] of the two arrays, which must be as long */
-    const uint32_t *bias_ids;     /* x + value; an id listed twice gets both, in the order of the list */
+                                   * bias_starts[r + 1] of the two lists below, which the caller answers for:
+                                   * both must be at least bias_starts[rows] long (a row that would end
+                                   * before it starts has none) */
+    const uint32_t *bias_ids;     /* x + the id's value; of an id listed twice the sum, in the list's order */
     const float *bias_values;
     const uint32_t *mask;         /* bit id % 32 of word id / 32 of a row: 0 makes the logit -infinity */
     uint64_t history_stride, mask_stride; /* elements and words from row to row; history_stride < 2^30 */

@@ -165,6 +165,22 @@ def test_biases_of_one_id_add_in_the_order_of_the_list(vk):
     assert float(out[0, 13]) == float(want)
 
 
+def test_a_row_whose_biases_end_before_they_start_has_none(vk):
+    """Starts that fall, all of them within the lists: rows 1 and 3 have no biases, the others theirs."""
+    import torch
+
+    c = case(5, 300, 4, 2, "f32")
+    c["bias_starts"] = np.array([6, 9, 2, 8, 0, 4], dtype=np.uint32)
+    c["bias_ids"] = np.arange(12, dtype=np.uint32) * 7
+    c["bias_values"] = np.arange(1, 13).astype(np.float32)
+    x = torch.from_numpy(c["x"]).cuda()
+    out = torch.zeros_like(x)
+    assert run(vk, torch, c, RULES["bias"], "f32", x, out) == vk.OK
+    ref, tol = reference(c, RULES["bias"])
+    assert (ref[[1, 3]] == c["x"][[1, 3]]).all() and (ref[[0, 2, 4]] != c["x"][[0, 2, 4]]).any(1).all()
+    close(out.cpu().numpy().astype(np.float64), ref, tol, "f32")
+
+
 def test_one_id_over_and_over(vk):
     """A history of one repeated id, in the prompt and after it, that is also biased."""
     import torch
