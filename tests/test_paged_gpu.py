@@ -673,6 +673,37 @@ def test_attention_flags_bad_pages_and_lengths(vk, torch, dtype):
     assert bool((a.out[4:] == 7.5).all())
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_flags_the_last_id_beside_the_largest_pool(vk, torch, dtype):
+    """2^32 - 1 pages (one above the other: their stride is 0), whose last id is 2^32 - 2: the id 2^32 - 1 is bad, and
+    has no key."""
+    dt = torch.float16 if dtype == "f16" else torch.float32
+    k, v, q = (torch.randn((1, 64), device="cuda").to(dt) for _ in range(3))
+    out, status = torch.zeros_like(q), torch.zeros(1, dtype=torch.int32, device="cuda")
+    kv = vk.PagedKV(k.data_ptr(), v.data_ptr(), 0, 64, 64, 0xffffffff, 1, 1, 64, vk.F16 if dtype == "f16" else vk.F32, 0)
+    table, lens = i32(torch, [5, 0xfffffffe, 7]), i32(torch, [3])
+    ws = torch.zeros(vk.PAGED_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+    t = vk.PagedTable(table.data_ptr(), None, 3, 1, 3, 1, 0xffffffff)
+
+    def call():
+        out.zero_()
+        status.zero_()
+        assert vk.lib().vkllm_b200_paged_attention(C.byref(kv), C.byref(t), q.data_ptr(), 64, 1, lens.data_ptr(), 0.125,
+                                                   out.data_ptr(), 64, ws.data_ptr(), ws.numel(), status.data_ptr(),
+                                                   stream(torch)) == vk.OK
+        torch.cuda.synchronize()
+        return int(status)
+
+    tol = (3 + 64 + 8) * 2 * U + 2.0 ** -21
+    assert call() == 0
+    within(out, v.double(), tol * v.double().abs() + out_tol(v.double(), dtype))
+    table[1] = -1
+    assert call() == vk.PAGED_BAD_PAGE
+    within(out, v.double(), tol * v.double().abs() + out_tol(v.double(), dtype))
+    table.fill_(-1)
+    assert call() == vk.PAGED_BAD_PAGE and bool((out == 0).all())
+
+
 def test_memory_that_is_not_the_devices_is_refused(vk, torch):
     """Every array of every call in turn as pinned host memory: refused, and nothing runs."""
     a = Attend(vk, torch, [20], 2, 2, 64, 16, "f16")

@@ -257,8 +257,8 @@ template <typename T, int KD, bool EXACT> struct Loader
         if (more(a) && key < c.len)
         {
             page = __ldg(a.table + c.seq * a.table_stride + col);
-            if (page == kNoPage) // (n_pages is below it)
-                page = kNoPage - 1;
+            if (page == kNoPage) // an id past every pool, however many pages that has
+                status |= VKLLM_B200_PAGED_BAD_PAGE;
         }
     }
     // At an item's first tile: where its keys lie, and its queries, which will be wanted, on their way to L1.
