@@ -43,7 +43,8 @@ enum
     VKLLM_B200_PAGED_TOO_MANY = 8,  /* append: more new tokens than max_tokens; release: more pages than n_pages */
     VKLLM_B200_PAGED_BAD_SLOT = 16, /* rope_write: a slot >= n_pages * page_rows other than NO_SLOT */
     VKLLM_B200_PAGED_BAD_WORKSPACE = 32, /* attention: the workspace was not zero at first, or two calls
-                                          * used it at the same time; rows of out are missing */
+                                          * used it at the same time; rows of out are missing, and the
+                                          * workspace has to be zeroed before its next use */
 };
 
 /* The page table of a batch of sequence slots. Row s of a sequence's cache is row s % page_rows of page
@@ -110,14 +111,15 @@ extern vkllm_err_t vkllm_b200_paged_release(const struct vkllm_b200_paged_table 
 
 /* RoPE of new tokens and their rows of the cache: q_out = rotated q, key row = rotated k, value row = v,
  * with the pairs and angles of VKLLM_OP_ROPE (elements 2w and 2w + 1 turned by positions[t] *
- * rope_base^(-2w / head_dim); src/shaders/vkllm_rope.comp), exact at far positions too.
+ * rope_base^(-2w / head_dim); src/shaders/vkllm_rope.comp). Sines and cosines are off by at most 2^-22, at
+ * far positions as at near ones.
  *   q [n_tokens] rows of heads * head_dim, k and v of kv_heads * head_dim, q_out as q; row strides in
  *   elements, multiples of 16 bytes, pointers 16-byte aligned: q, k and v may be parts of one row.
  *   heads a multiple of kv_heads; rope_base > 1 (<= 0: 10000). q_out may be q (same stride); it must not
  *   overlap q, k or v otherwise.
- * A token whose slot is VKLLM_B200_NO_SLOT leaves the cache and its q_out row as they were; so does a
- * slot outside the pool, which sets VKLLM_B200_PAGED_BAD_SLOT. The other slots must differ. n_tokens may
- * be 0. */
+ * A token whose slot is VKLLM_B200_NO_SLOT leaves the cache and its q_out row as they were, and its rows
+ * are not read; a token whose slot is outside the pool leaves both as they were and sets
+ * VKLLM_B200_PAGED_BAD_SLOT. The other slots must differ. n_tokens may be 0. */
 extern vkllm_err_t vkllm_b200_paged_rope_write(const struct vkllm_b200_paged_kv *kv, const void *q, uint64_t q_stride,
                                                const void *k, uint64_t k_stride, const void *v, uint64_t v_stride,
                                                const uint32_t *positions, const uint32_t *slots, uint32_t n_tokens,
@@ -168,7 +170,11 @@ struct vkllm_b200_logit_rules
     const uint32_t *bias_ids;     /* x + the id's value; of an id listed twice the sum, in the list's order */
     const float *bias_values;
     const uint32_t *mask;         /* bit id % 32 of word id / 32 of a row: 0 makes the logit -infinity */
-    uint64_t history_stride, mask_stride; /* elements and words from row to row; history_stride < 2^30 */
+    uint64_t history_stride, mask_stride; /* elements and words from row to row; history_stride < 2^30.
+                                           * A stride past 2560 sets twice the shared memory aside, whatever
+                                           * the lengths. More than 6144 entries of history and biases (3072
+                                           * up to that stride) are read again for every 8192 (4096) ids of
+                                           * vocab */
 };
 
 /* out = logits under the rules, in the order of the struct (repetition, frequency and presence, biases,

@@ -1,4 +1,4 @@
-// Attention of one new token per sequence over a paged KV cache.
+// Attention of one query row per row of a page table (a sequence, or a token of one) over a paged KV cache.
 //
 //   out = sum_j exp(scale q . k_j - m) v_j / sum_j exp(scale q . k_j - m),  j < len,  m = max_j scale q . k_j
 //
@@ -13,8 +13,8 @@
 // over all SMs and short ones share a CTA. A CTA that holds only a part of an item leaves (m, l, O) in the
 // workspace and counts itself at the item; the last one to arrive joins the parts in the order of the line,
 // so the result does not depend on who was last. (Handing the last quarter of the line out in small chunks
-// off a ticket counter was slower: 98 instead of 78 us for 64 sequences of 128 to 640 keys, since every
-// chunk refills the rings.)
+// off a ticket counter was slower: 98 us for 64 sequences of 128 to 640 keys, where equal parts took 78 then and
+// take 67 now, since every chunk refills the rings.)
 //
 // Loads. Each warp streams its own slices through a private ring of cp.async stages, also across the
 // borders of items: no barrier of the CTA stands between a load and its use. Page ids are read one tile
@@ -83,7 +83,8 @@ template <typename T, int KD> struct Shape
     // the same bytes: 8 x 16 heads of 64 with 4096 keys take 31.7 us with 3 CTAs of 4 stages, 35.9 with 2 of 6; 28
     // heads of 80 over 4 take 72 with 3 of 2 and 80 with 2 of 3. Of 128, 3 CTAs of 2 stages (kRound 2) are better
     // where items are short (200 sequences of up to 120 keys: 48 instead of 57 us) and worse where they are long or
-    // 16 queries share a head (65 instead of 59), so it stays at 2 of 3.
+    // 16 queries share a head (65 instead of 59), so it stays at 2 of 3. With 3 CTAs a thread has 168 registers, which
+    // costs most kernels of up to 96 dimensions 8 to 60 bytes of spills; the times above include them.
     static constexpr uint32_t kStages = KD <= 64 ? (sizeof(T) == 4 ? 3 : 4) : sizeof(T) == 4 || KD == 96 ? 2 : 3;
     static constexpr uint32_t kCtas = KD > 128 ? 1 : KD <= 96 ? 3 : 2;
     static constexpr uint32_t kRound = 4;
@@ -232,7 +233,9 @@ template <typename T, int KD, bool EXACT> struct Loader
     uint32_t stage = 0, status = 0;
     uint32_t pieces, row0, p0, drow, dp; // the copies of a lane: pieces of a row, its first one, from one to the next
     const char *k, *v;                   // the pools (at the lane's piece where that is fixed)
-    uint64_t policy; // rows are read once: they leave L2 first, and what others have there stays (1 to 5% faster)
+    // rows are read once: they leave L2 first, and what others have there stays (one sequence of 131072 92.4 -> 91.1 us,
+    // 64 of 128 to 640 74.3 -> 72.5, when that was measured)
+    uint64_t policy;
 
     __device__ __forceinline__ void begin(const PagedAttArgs &a, uint32_t warp, uint32_t lane)
     {

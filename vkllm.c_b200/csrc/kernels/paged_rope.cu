@@ -9,18 +9,20 @@
 // Angles: fp32 loses the angle of far positions (at position 200000 the rounding of position * frequency
 // alone is 8e-3 radians). The frequency is kept as a fraction of a turn in 64-bit fixed point, f =
 // base^(-2w / hd) / (2 pi) < 2^-2, so position * f modulo 2^64 is the exact fraction of the last turn for
-// the rounded f: an error of at most position * 2^-64 turns, and no range reduction. sincospif takes it
-// from there in fp32.
+// the rounded f: an error of at most position * 2^-64 turns, and no range reduction. Rounded to fp32 as a
+// number of half turns it is off by up to 2^-25 of one, which moves a sine by up to 9.4e-8, at near positions
+// as at far ones. With fp32 rows that shows (5.5e-8 of the outputs' size from 64 bits, where a sine of a 64-bit
+// angle gives 4.2e-8), with fp16 rows it does not.
 //
 // A block works out a token's sines and cosines once, into shared memory; each thread owns one 16-byte
 // piece of a head (4 or 2 pairs), keeps those of its pairs, and walks over its share of the token's heads,
 // kAhead loads in flight, the first of them on their way before the position and the sines are known. 2048
-// tokens of 40 + 80 heads of 128 (126 MB, fp16): 20.4 us, 6.2 TB/s (24.6 with the loads after the sines, 27.5
+// tokens of 40 + 80 heads of 128 (126 MB, fp16): 21.6 us, 5.8 TB/s (24.6 with the loads after the sines, 27.5
 // with sines worked out by every thread), where a plain copy of 102 MB reaches 5.5.
 //
 // The loads wait for the slot: a step that is launched for the most tokens it may have is mostly padding, whose
 // rows are not read. 64 tokens among 8192, 32 + 16 heads of 128: 5.5 us; 20.6 where the loads go out first, which
-// gives 64 tokens without padding 2.6 us instead of 2.7, 2048 of 32 + 16 heads 10.2 instead of 10.5 and longer
+// gives 64 tokens without padding 2.65 us instead of 2.80, 2048 of 32 + 16 heads 10.2 instead of 10.5 and longer
 // calls nothing.
 #include <cmath>
 
@@ -47,8 +49,9 @@ struct RopeArgs
 };
 
 // 16 bytes as fp32 pairs. kAhead: rows of a thread in flight; kCtas: blocks of an SM that the registers are kept
-// to. fp16 2048 tokens of 40 + 80 heads take 20.4 us with 4 x 6 blocks, 21.5 with 4 x 5, 21.8 with 3 x 8, 23.1 with
-// 4 x 8 (registers spill); fp32 1500 tokens of 32 + 16 heads 12.5 with 3 x 8, 13.4 with 4 x 6.
+// to. fp16, 2048 tokens of 40 + 80 heads, three sets of rows into one pool: 20.4 us with 4 x 6 blocks, 21.5 with
+// 4 x 5, 21.8 with 3 x 8, 23.1 with 4 x 8 (registers spill); fp32, 1500 tokens of 32 + 16 heads: 12.5 with 3 x 8,
+// 13.4 with 4 x 6.
 template <typename T> struct Piece;
 template <> struct Piece<__half>
 {
