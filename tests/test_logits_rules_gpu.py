@@ -128,6 +128,19 @@ def test_rules(vk, dtype, on, rows, vocab, past, bias, pad):
     assert torch.equal(y[:, vocab:], x[:, vocab:])
 
 
+@pytest.mark.parametrize("on", ["all", "mask", "nothing"])
+def test_the_most_rows(vk, on):
+    import torch
+
+    c = case(65535, 23, 5, 6, "f16", 2, 1)
+    x = torch.from_numpy(c["x"]).cuda()
+    out = torch.full((65535, 24), 9.0, dtype=x.dtype, device="cuda")
+    assert run(vk, torch, c, RULES[on], "f16", x, out) == vk.OK
+    ref, tol = reference(c, RULES[on])
+    close(out[:, :23].cpu().numpy().astype(np.float64), ref, tol, "f16")
+    assert bool((out[:, 23:] == 9.0).all())
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("shift_in,shift_out", [(0, 0), (1, 1), (3, 3), (1, 2), (5, 0)])
 def test_rows_at_every_alignment(vk, dtype, shift_in, shift_out):

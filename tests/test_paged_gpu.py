@@ -775,6 +775,32 @@ def test_attention_keeps_infinities_where_they_are(vk, torch, dtype):
     within(got[1, :4], p @ v, 2.0 ** -11 * (p @ v).abs() + 2.0 ** -16 * (p @ v.abs()) + 2.0 ** -25)
 
 
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("hd", [4, 12, 36, 68, 100, 196, 252])
+def test_fp32_heads_of_an_odd_number_of_pieces(vk, torch, layout, hd):
+    """fp32 head sizes that are multiples of 4 and not of 8, through RoPE and attention."""
+    test_rope_write(vk, torch, "f32", layout, 6, 3, hd, 37, 7, 10000.0)
+    for lens in (LENS["few"], LENS["long"]):
+        a = Attend(vk, torch, lens, 10, 2, hd, 7, "f32", layout, seed=hd)
+        assert a.call() == vk.OK
+        a.check(f"heads of {hd}")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_whose_every_score_is_minus_infinity(vk, torch, dtype):
+    """Rows of zeros for the heads of a key head that scores so throughout, in one part of a CTA and in parts of
+    many; the other key head's are as ever."""
+    a = Attend(vk, torch, [50, 40000, 1, 0, 300], 8, 2, 64, 16, dtype, seed=15)
+    a.q[:, :512] = a.q[:, :512].abs() + 0.1
+    a.k[:, 0, :, 7] = -float("inf")
+    assert a.call() == vk.OK
+    torch.cuda.synchronize()
+    ref, tol = a.reference()
+    got = a.out[:5, :512].reshape(5, 8, 64)
+    assert int(a.status) == 0 and bool((got[:, :4] == 0).all())
+    within(got[:, 4:], ref[:, 4:], tol[:, 4:])
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_attention_of_the_most_sequences(vk, torch, dtype):
     """65535 slots of none to three rows, a page each: many sequences for every thread of the division, and
