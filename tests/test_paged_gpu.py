@@ -417,6 +417,30 @@ def test_rope_write(vk, torch, dtype, layout, H, HK, hd, n, page_rows, base):
     assert torch.equal(v.double(), refv)
 
 
+@pytest.mark.parametrize("hd,base", [(128, 10000.0), (256, 1000000.0), (8, 1.5)])
+def test_rope_sines_at_far_positions(vk, torch, hd, base):
+    """Queries of (1, 0) pairs in fp32 come out as the cosines and sines themselves. Tolerance 2^-22: the angle as a
+    number of half turns in fp32 is off by 2^-25 of one, a sine by pi times that (9.4e-8), and sincospif by 2 units in the
+    last place of values below 1 (1.2e-7). The reference's angle, with 64 bits of mantissa, is off by 2^-33."""
+    assert np.finfo(np.longdouble).nmant >= 63
+    n = 4096
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    k, v, kv = make_pools(vk, torch, "heads first", 1, n, 1, hd, "f32", g)
+    qkv = torch.zeros((n, 3 * hd), device="cuda")
+    qkv[:, 0:hd:2] = 1
+    positions = np.random.default_rng(hd).integers(0, 2 ** 31, n)
+    positions[:3] = 0, 1, 2 ** 31 - 1
+    q_out, status = torch.zeros((n, hd), device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    slots = torch.arange(n, device="cuda", dtype=torch.int32)
+    assert rope_call(vk, torch, kv, qkv, 1, 1, hd, i32(torch, positions), slots, n, base, q_out, status) == vk.OK
+    got = q_out.cpu().numpy().astype(np.longdouble)
+    w = np.arange(hd // 2, dtype=np.longdouble)
+    th = positions.astype(np.longdouble)[:, None] * np.longdouble(np.float32(base)) ** (-2 * w / hd)
+    assert int(status) == 0
+    assert float(np.abs(got[:, 0::2] - np.cos(th)).max()) <= 2.0 ** -22
+    assert float(np.abs(got[:, 1::2] - np.sin(th)).max()) <= 2.0 ** -22
+
+
 def test_rope_write_in_place_equals_out_of_place(vk, torch):
     g = torch.Generator(device="cuda").manual_seed(5)
     H, HK, hd, n = 8, 2, 64, 40

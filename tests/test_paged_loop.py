@@ -1,5 +1,5 @@
-"""The serving loop of INTEGRATION.md, compiled as it stands there: on the CPU that it compiles, on the GPU what it
-computes for steps in which slots wait, decode, get prompts, end and start again, called and replayed."""
+"""The documented serving loop, compiled as it stands in the integration notes: on the CPU that it compiles, on the
+GPU what it computes for steps in which slots wait, decode, get prompts, end and start again, called and replayed."""
 import ctypes as C
 import os
 import subprocess
