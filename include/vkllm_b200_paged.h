@@ -172,9 +172,9 @@ struct vkllm_b200_logit_rules
     const uint32_t *mask;         /* bit id % 32 of word id / 32 of a row: 0 makes the logit -infinity */
     uint64_t history_stride, mask_stride; /* elements and words from row to row; history_stride < 2^30.
                                            * A stride past 2560 sets twice the shared memory aside, whatever
-                                           * the lengths. More than 6144 entries of history and biases (3072
-                                           * up to that stride) are read again for every 8192 (4096) ids of
-                                           * vocab */
+                                           * the lengths, for 8192 ids instead of 4096. A row's history and
+                                           * biases that take more than 3/4 of these are read again for every
+                                           * 8192 (4096) ids of vocab */
 };
 
 /* out = logits under the rules, in the order of the struct (repetition, frequency and presence, biases,
